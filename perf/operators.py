@@ -249,7 +249,7 @@ def _plan(s):
     upto = need.cumsum(0)
     free = s["num_free"].long()
     admitted = fits & ((need == 0) | (upto <= free))
-    used = torch.where(admitted, upto, 0).amax()
+    used = torch.where(admitted & (need > 0), upto, 0).amax()
     column = torch.arange(table.shape[1], device=table.device)[None]
     fresh = admitted[:, None] & (column >= have[:, None]) & (column < want[:, None])
     source = free - 1 - ((upto - need)[:, None] + column - have[:, None])
