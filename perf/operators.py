@@ -183,7 +183,7 @@ def prepare(case, seed):
         table[held] = order[: sum(have)]
         free = order[sum(have):].contiguous()
         state.update(context_lens=_ints(cached), cu_seqlens=_ints(_cumulated(new)), block_table=table,
-                     free_blocks=free, num_free=_ints([free.numel()]), total=sum(new), page=page, parents=None, words=0)
+                     held_blocks=_ints(have), free_blocks=free, num_free=_ints([free.numel()]), total=sum(new), page=page, parents=None, words=0)
         if case["tree"]:
             state.update(parents=_ints(sum(_parents(case, new), [])), words=-(-case["tokens"] // 32))
         return state
@@ -243,7 +243,8 @@ def prepare(case, seed):
 def _plan(s):
     ctx, cu, table, page = s["context_lens"].long(), s["cu_seqlens"].long(), s["block_table"], s["page"]
     new = cu[1:] - cu[:-1]
-    have, want = (ctx + page - 1) // page, (ctx + new + page - 1) // page
+    have = s["held_blocks"].long()
+    want = torch.maximum(have, (ctx + new + page - 1) // page)
     fits = want <= table.shape[1]
     need = torch.where(fits, want - have, 0)
     upto = need.cumsum(0)
@@ -260,8 +261,9 @@ def _plan(s):
     place = ctx[request] + index
     slot = table[request, (place // page).clamp(max=table.shape[1] - 1)].long() * page + place % page
     slots = torch.where(admitted[request], slot, -1)
+    left, held = (free - used).int(), torch.where(admitted, want, have).int()
     if s["parents"] is None:
-        return table, slots, place.int(), admitted, (free - used).int(), None
+        return table, slots, place.int(), admitted, left, held, None
     width = 32 * s["words"]
     above = torch.zeros(new.numel(), width, width, device=table.device)
     inner = s["parents"] >= 0
@@ -273,7 +275,7 @@ def _plan(s):
     positions = ctx[request] + rows.sum(1) - 1
     bits = (rows.view(-1, s["words"], 32) << torch.arange(32, device=table.device)).sum(2)
     mask = torch.where(bits >= 1 << 31, bits - (1 << 32), bits).int()
-    return table, slots, positions.int(), admitted, (free - used).int(), mask
+    return table, slots, positions.int(), admitted, left, held, mask
 
 
 def _rotated(x, cos, sin, rot, interleaved):
@@ -369,10 +371,10 @@ def run(state):
     from flashlite_b200 import flash_attn_wmma as fa
 
     if c["op"] == "plan":
-        slots, positions, admitted, left, mask = fa.plan_cache_step(
-            s["context_lens"], s["cu_seqlens"], s["block_table"], s["free_blocks"], s["num_free"], s["total"], s["page"],
-            parents=s["parents"], mask_words=s["words"])
-        return s["block_table"], slots, positions, admitted, left, mask
+        slots, positions, admitted, left, held, mask = fa.plan_cache_step(
+            s["context_lens"], s["cu_seqlens"], s["block_table"], s["held_blocks"], s["free_blocks"], s["num_free"],
+            s["total"], s["page"], parents=s["parents"], mask_words=s["words"])
+        return s["block_table"], slots, positions, admitted, left, held, mask
     if c["op"] == "rotary":
         more = dict(interleaved=c["interleaved"], layout=c["layout"])
         q, k = fa.rotary(s["q"], s["k"], s["table"], s["positions"], **more)
@@ -398,7 +400,7 @@ def work(case):
         fresh = sum(-(-(c + x) // case["page"]) + (-c // case["page"]) for c, x in zip(cached, new))
         words = -(-case["tokens"] // 32) if case["tree"] else 0
         # lengths and offsets read, fresh blocks read and written, a slot and a position for each token, parents and masks
-        return {"bytes": n * (4 + 4 + 1) + 8 * fresh + 12 * t + (4 + 4 * words) * t * case["tree"], "flops": 4 * t}
+        return {"bytes": n * (4 + 4 + 4 + 4 + 1) + 8 * fresh + 12 * t + (4 + 4 * words) * t * case["tree"], "flops": 4 * t}
     size = 4 if case["dtype"] == "fp32" else 2
     heads, kv_heads, dim = case["heads"], case["kv_heads"], case["dim"]
     if op == "rotary":
