@@ -24,7 +24,8 @@ INCLUDE = PKG.parent / "include"
 BUILD = PKG / "_build"
 
 CUDA_SOURCES = ["fl_api.cu", "fl_flash2.cu", "fl_flash2_sk.cu", "fl_flash2_bwd.cu", "fl_naive.cu",
-                "fl_noalloc.cu", "fl_selftest.cu"]
+                "fl_noalloc.cu", "fl_selftest.cu", "fl_rotary.cu", "fl_plan.cu", "fl_tree.cu"]
+BINDING_SOURCES = ["flash_attn.cpp", "serving.cpp"]
 HEADERS = ["fl_ptx.cuh", "fl_internal.h", "fl_flash2_common.cuh"]
 LIB = PKG / "libflashlite_b200.so"
 EXT = PKG / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
@@ -92,21 +93,31 @@ def build_library(verbose: bool = False) -> Path:
 
 
 def build_binding(verbose: bool = False) -> Path:
-    """Compile the torch binding (flash_attn.cpp) against libflashlite_b200.so."""
+    """Compile the torch binding (BINDING_SOURCES) against libflashlite_b200.so."""
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = CSRC / "flash_attn.cpp"
-    if not _stale(EXT, [src, INCLUDE / "flashlite_b200.h", LIB, Path(__file__)]):
+    srcs = [CSRC / s for s in BINDING_SOURCES]
+    if not _stale(EXT, [*srcs, INCLUDE / "flashlite_b200.h", LIB, Path(__file__)]):
         return EXT
     cxx = os.environ.get("CXX", "g++")
     incs = ce.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"]]
     libdirs = ce.library_paths(device_type="cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
-           "-DTORCH_API_INCLUDE_EXTENSION_H",
-           *[f"-I{p}" for p in incs], str(src), "-o", str(EXT),
+    flags = ["-O2", "-std=c++17", "-fPIC", "-w",
+             f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
+             "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{p}" for p in incs]]
+    BUILD.mkdir(exist_ok=True)
+
+    def compile_one(src):
+        obj = BUILD / (src.name + ".o")
+        if _stale(obj, [src, INCLUDE / "flashlite_b200.h", Path(__file__)]):
+            _run([cxx, *flags, "-c", str(src), "-o", str(obj)], BUILD / (src.name + ".log"))
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(srcs)) as ex:
+        objs = list(ex.map(compile_one, srcs))
+    cmd = [cxx, "-shared", *map(str, objs), "-o", str(EXT),
            *[f"-L{p}" for p in libdirs], f"-L{PKG}",
            "-lflashlite_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
            "-ltorch_python", "-lcudart",

@@ -16,6 +16,7 @@
 
 #include "../../include/flashlite_b200.h"
 #include "fl_internal.h"
+#include "fl_ptx.cuh"
 
 namespace fl {
 
@@ -73,18 +74,38 @@ int sm_count() {
   return (dev >= 0 && dev < kMaxDevices && g_sm_count[dev] > 0) ? g_sm_count[dev] : 148;
 }
 
-}  // namespace fl
-
-namespace {
-
 int fail(int status, const std::string& msg) {
-  fl::set_last_error(msg);
+  set_last_error(msg);
   return status;
 }
 
 int cuda_fail(cudaError_t e, const char* where) {
   return fail(FL_ERR_CUDA, std::string(where) + ": " + cudaGetErrorString(e));
 }
+
+int check_device() {
+  const int dev = current_device();
+  if (dev < 0) return fail(FL_ERR_NO_DEVICE, "no CUDA device");
+  // Bind the device's primary context to this thread: tensor maps are encoded
+  // through the driver API before the first runtime launch, and a thread
+  // that has only queried the device (an autograd worker, say) has no
+  // current context yet.
+  if (cudaSetDevice(dev) != cudaSuccess) return fail(FL_ERR_NO_DEVICE, "cannot bind the CUDA device");
+  if (!init_device(dev)) return fail(FL_ERR_CUDA, "device initialisation failed");
+  int major = 0;
+  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+  if (major != 10) return fail(FL_ERR_NO_DEVICE, "flashlite_b200 kernels are built for sm_100a (B200)");
+  return FL_OK;
+}
+
+}  // namespace fl
+
+namespace {
+
+using fl::aligned16;
+using fl::check_device;
+using fl::cuda_fail;
+using fl::fail;
 
 // Checks shared by the attention entry points; returns FL_OK or an error.
 int check_common(const void* q, const void* k, const void* v, const void* o, int64_t B, int64_t H,
@@ -101,23 +122,6 @@ int check_common(const void* q, const void* k, const void* v, const void* o, int
   return FL_OK;
 }
 
-int check_device() {
-  const int dev = fl::current_device();
-  if (dev < 0) return fail(FL_ERR_NO_DEVICE, "no CUDA device");
-  // Bind the device's primary context to this thread: tensor maps are encoded
-  // through the driver API before the first runtime launch, and a thread
-  // that has only queried the device (an autograd worker, say) has no
-  // current context yet.
-  if (cudaSetDevice(dev) != cudaSuccess) return fail(FL_ERR_NO_DEVICE, "cannot bind the CUDA device");
-  if (!fl::init_device(dev)) return fail(FL_ERR_CUDA, "device initialisation failed");
-  int major = 0;
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-  if (major != 10) return fail(FL_ERR_NO_DEVICE, "flashlite_b200 kernels are built for sm_100a (B200)");
-  return FL_OK;
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 }  // namespace
 
 extern "C" {
@@ -133,6 +137,7 @@ const char* fl_status_str(int status) {
     case FL_ERR_CUDA: return "CUDA error";
     case FL_ERR_NO_DEVICE: return "no sm_100 device";
     case FL_ERR_DEVICE_TIMEOUT: return "a kernel wait timed out";
+    case FL_ERR_DEVICE_INDEX: return "a kernel met an index out of range";
     default: return "unknown status";
   }
 }
@@ -293,7 +298,8 @@ int fl_device_error(void* stream, uint32_t* flags) {
     cudaMemcpyToSymbol(fl::g_device_error, &zero, sizeof(zero));
   }
   if (flags) *flags = word;
-  return word ? fail(FL_ERR_DEVICE_TIMEOUT, "a kernel gave up a bounded wait") : FL_OK;
+  if (word & fl::kDevErrWaitTimeout) return fail(FL_ERR_DEVICE_TIMEOUT, "a kernel gave up a bounded wait");
+  return word ? fail(FL_ERR_DEVICE_INDEX, "a kernel met an index outside its table") : FL_OK;
 }
 
 }  // extern "C"

@@ -13,6 +13,43 @@ namespace fl {
 void set_last_error(const std::string& msg);
 const char* last_error();
 
+// Helpers of the C entry points: set the error text and return the status,
+// bind and check the current device, test a pointer's alignment.
+int fail(int status, const std::string& msg);
+int cuda_fail(cudaError_t e, const char* where);
+int check_device();
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Runs the body of a C entry point; nothing it throws (an allocation of the
+// error text, say) leaves the C interface.
+template <typename Body>
+int guarded(Body&& body) noexcept {
+  try {
+    return body();
+  } catch (...) {
+    return 4;  // FL_ERR_CUDA; no text, as the text may be what failed
+  }
+}
+
+// Launch with programmatic stream serialization: the kernel may start while
+// the previous one on the stream drains, and waits for its results itself
+// (griddepcontrol.wait before the first access to global memory).
+template <typename Params>
+cudaError_t launch_pdl(void (*kern)(Params), int blocks, int threads, int smem, cudaStream_t stream,
+                       const Params& prm) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, prm);
+}
+
 // Device-side error word of the current device (address in device memory).
 unsigned int* device_error_word();
 

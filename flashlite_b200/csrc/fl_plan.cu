@@ -1,0 +1,229 @@
+// Bookkeeping of one serving step: block-table entries, slots and positions
+// of the new tokens, ancestor masks of drafted trees.
+//
+//   have_b = max(held_b, ceil(ctx_b / page)), want_b = max(have_b, ceil((ctx_b + T_b) / page))
+//   need_b = want_b - have_b (0 if the row is too short), upto = prefix sum
+//   admitted_b = row long enough and (need_b == 0 or upto_b <= num_free)
+//   block j of request b, have_b <= j < want_b:
+//     free[num_free - 1 - (upto_b - need_b + j - have_b)]
+//
+// Bound by latency: a few bytes per request and token. One launch: every
+// block computes the prefix sum over all requests again (8 bytes of shared
+// memory per request) rather than a first kernel handing it to a second, and
+// then serves its own share of the tokens (one thread each) and of the
+// requests' table rows (one warp each). A token takes a fresh block's number
+// from the free list itself, so no block waits for another's table entries.
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+#include "../../include/flashlite_b200.h"
+#include "fl_internal.h"
+#include "fl_ptx.cuh"
+
+namespace fl {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxRequests = 16384;
+
+struct PlanParams {
+  fl_plan_args a;
+  unsigned int* err;
+};
+
+struct Request {
+  int begin, count, ctx, have, need;
+  bool fits;
+};
+
+// Request b's share of the arithmetic above. Lengths out of range count as
+// none and are recorded.
+__device__ __forceinline__ Request request_of(const PlanParams& p, int b, bool report) {
+  const fl_plan_args& a = p.a;
+  Request r;
+  r.ctx = a.context_lens[b];
+  r.begin = a.cu_seqlens[b];
+  const int end = a.cu_seqlens[b + 1];
+  const bool sound = r.ctx >= 0 && r.begin >= 0 && end >= r.begin && end <= a.tokens &&
+                     r.ctx <= 0x7fffffff - (end - r.begin) - static_cast<int>(a.page_size);
+  if (!sound) {
+    if (report && p.err) atomicOr(p.err, kDevErrIndex);
+    r.ctx = r.begin = r.count = r.have = r.need = 0;
+    r.fits = false;
+    return r;
+  }
+  r.count = end - r.begin;
+  const int page = static_cast<int>(a.page_size);
+  r.have = max(a.held_blocks[b], (r.ctx + page - 1) / page);
+  const int want = max(r.have, (r.ctx + r.count + page - 1) / page);
+  r.fits = want <= a.table_cols;
+  r.need = r.fits ? want - r.have : 0;
+  return r;
+}
+
+__global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ PlanParams p) {
+  extern __shared__ int smem[];
+  const fl_plan_args& a = p.a;
+  const int nb = static_cast<int>(a.requests);
+  int* s_first = smem;           // [nb] blocks taken by the requests before; -1: refused
+  int* s_cu = smem + nb;         // [nb + 1]
+  __shared__ long long s_warp[kThreads / 32];
+  __shared__ int s_used;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- prefix sum of the blocks needed: each thread takes a run of requests ----
+  const int per = (nb + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, nb), b1 = min(b0 + per, nb);
+  // blocks that are not there cannot be given out
+  const int free_n = max(0, min(a.num_free[0], static_cast<int>(a.free_capacity)));
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += request_of(p, b, blockIdx.x == 0).need;
+  long long incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += x;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  if (tid == 0) {
+    s_used = 0;
+    s_cu[nb] = a.cu_seqlens[nb];
+  }
+  __syncthreads();
+  long long upto = incl - mine;
+  for (int w = 0; w < warp; ++w) upto += s_warp[w];
+  int used = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Request r = request_of(p, b, false);
+    const bool admitted = r.fits && (r.need == 0 || upto + r.need <= free_n);
+    s_first[b] = !admitted ? -1 : r.need > 0 ? static_cast<int>(upto) : 0;
+    s_cu[b] = a.cu_seqlens[b];
+    upto += r.need;
+    if (admitted && r.need > 0) used = static_cast<int>(upto);
+    if (blockIdx.x == 0) {
+      a.admitted[b] = admitted ? 1 : 0;
+      a.held_after[b] = r.have + (admitted ? r.need : 0);
+    }
+  }
+  if (blockIdx.x == 0 && used > 0) atomicMax(&s_used, used);
+  __syncthreads();
+  if (blockIdx.x == 0 && tid == 0) a.num_free_after[0] = free_n - s_used;
+
+  // ---- table rows: one warp per request ----
+  const int page = static_cast<int>(a.page_size);
+  for (int b = blockIdx.x * (kThreads / 32) + warp; b < nb; b += gridDim.x * (kThreads / 32)) {
+    const int first = s_first[b];
+    if (first < 0) continue;
+    const Request r = request_of(p, b, false);
+    int32_t* row = a.block_table + static_cast<int64_t>(b) * a.table_stride + r.have;
+    for (int j = lane; j < r.need; j += 32) row[j] = a.free_blocks[free_n - 1 - first - j];
+  }
+
+  // ---- tokens: one thread each ----
+  const int total = static_cast<int>(a.tokens);
+  for (int t = blockIdx.x * kThreads + tid; t < total; t += gridDim.x * kThreads) {
+    // the last request that begins at or before t and is not empty there
+    int lo = 0, hi = nb;  // cu[lo] <= t < cu[hi] as far as it is known
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_cu[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    int64_t slot = -1;
+    int pos = 0;
+    const Request r = nb > 0 ? request_of(p, lo, false) : Request{0, 0, 0, 0, 0, false};
+    const int i = t - r.begin;
+    const bool inside = nb > 0 && i >= 0 && i < r.count;
+    if (inside) {
+      pos = r.ctx + i;
+      const int first = s_first[lo];
+      if (first >= 0) {
+        const int j = pos / page;
+        const int block = j < r.have ? a.block_table[static_cast<int64_t>(lo) * a.table_stride + j]
+                                     : a.free_blocks[free_n - 1 - first - (j - r.have)];
+        slot = static_cast<int64_t>(block) * page + pos % page;
+      }
+    }
+    a.slots[t] = slot;
+    if (a.parents != nullptr) {
+      // Ancestors have falling indices: each mask word is complete when the
+      // walk leaves it.
+      uint32_t* row = a.tree_mask + static_cast<int64_t>(t) * a.mask_words;
+      const int words = static_cast<int>(a.mask_words);
+      int next = words - 1, depth = -1;  // next: highest word not yet written
+      if (inside && i >= 32 * words) {
+        if (p.err) atomicOr(p.err, kDevErrIndex);
+      } else if (inside) {
+        int node = i, word = i >> 5;
+        uint32_t bits = 0;
+        while (node >= 0) {
+          if ((node >> 5) != word) {
+            while (next > word) row[next--] = 0u;
+            row[next--] = bits;
+            word = node >> 5;
+            bits = 0;
+          }
+          bits |= 1u << (node & 31);
+          ++depth;
+          const int up = a.parents[r.begin + node];
+          if (up >= node || up < -1) {  // not a tree: taken as a root
+            if (p.err) atomicOr(p.err, kDevErrIndex);
+            break;
+          }
+          node = up;
+        }
+        while (next > word) row[next--] = 0u;
+        row[next--] = bits;
+      }
+      while (next >= 0) row[next--] = 0u;
+      if (inside) pos = r.ctx + max(depth, 0);
+    }
+    a.positions[t] = pos;
+  }
+}
+
+int plan(const fl_plan_args* args, void* stream) {
+  if (args == nullptr) return fail(FL_ERR_INVALID_ARGUMENT, "null argument block");
+  const fl_plan_args& a = *args;
+  if (a.requests < 0 || a.tokens < 0 || a.table_cols < 0 || a.free_capacity < 0 || a.mask_words < 0)
+    return fail(FL_ERR_INVALID_ARGUMENT, "negative size");
+  if (a.page_size <= 0 || a.page_size > (1LL << 20))
+    return fail(FL_ERR_INVALID_ARGUMENT, "page_size must be positive");
+  if (a.requests > kMaxRequests) return fail(FL_ERR_UNSUPPORTED, "at most 16384 requests");
+  if (a.tokens > (1LL << 30) || a.table_cols > (1LL << 30) || a.free_capacity > 0x7fffffffLL ||
+      a.mask_words > (1LL << 20))
+    return fail(FL_ERR_INVALID_ARGUMENT, "dimension too large");
+  if (!a.cu_seqlens || !a.num_free || !a.num_free_after ||
+      (a.requests > 0 && (!a.context_lens || !a.held_blocks || !a.admitted || !a.held_after || (a.table_cols > 0 && !a.block_table))) ||
+      (a.free_capacity > 0 && !a.free_blocks) || (a.tokens > 0 && (!a.slots || !a.positions)))
+    return fail(FL_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (a.parents != nullptr && a.tokens > 0 && (a.mask_words == 0 || !a.tree_mask))
+    return fail(FL_ERR_INVALID_ARGUMENT, "a tree needs mask_words > 0 and a tree_mask");
+  int st = check_device();
+  if (st != FL_OK) return st;
+  PlanParams p;
+  p.a = a;
+  p.err = device_error_word();
+  const int smem = static_cast<int>(2 * a.requests + 1) * 4;
+  static std::atomic<bool> configured[kMaxFlagDevices];
+  cudaError_t e = ensure_smem_limit(plan_kernel, (2 * kMaxRequests + 1) * 4, configured);
+  if (e != cudaSuccess) return cuda_fail(e, "plan launch");
+  const int64_t want = std::max<int64_t>((a.tokens + kThreads - 1) / kThreads,
+                                         (a.requests + kThreads / 32 - 1) / (kThreads / 32));
+  const int blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, sm_count())));
+  e = launch_pdl(plan_kernel, blocks, kThreads, smem, static_cast<cudaStream_t>(stream), p);
+  return e == cudaSuccess ? FL_OK : cuda_fail(e, "plan launch");
+}
+
+}  // namespace
+}  // namespace fl
+
+extern "C" int fl_plan_cache_step(const fl_plan_args* args, void* stream) {
+  return fl::guarded([&] { return fl::plan(args, stream); });
+}

@@ -18,6 +18,7 @@ namespace fl {
 // Bit flags OR-ed into the device error word when a kernel gives up.
 enum : uint32_t {
   kDevErrWaitTimeout = 1u << 0,  // an mbarrier wait ran past its limit
+  kDevErrIndex = 1u << 1,        // a position, slot, block or length out of range: skipped
 };
 
 // A wait on an mbarrier that has not completed after this long is treated as

@@ -197,7 +197,7 @@ int64_t device_error() {
   uint32_t flags = 0;
   const int st = fl_device_error(
       static_cast<void*>(c10::cuda::getCurrentCUDAStream().stream()), &flags);
-  TORCH_CHECK(st == FL_OK || st == FL_ERR_DEVICE_TIMEOUT, "flashlite_b200: ", fl_status_str(st),
+  TORCH_CHECK(st == FL_OK || st == FL_ERR_DEVICE_TIMEOUT || st == FL_ERR_DEVICE_INDEX, "flashlite_b200: ", fl_status_str(st),
               ": ", fl_last_error());
   return static_cast<int64_t>(flags);
 }
@@ -240,6 +240,8 @@ std::vector<torch::Tensor> backward_flash2(torch::Tensor q, torch::Tensor k, tor
 
 }  // namespace
 
+void bind_serving(pybind11::module_& m);  // serving.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "FlashAttention-2 forward for B200 (sm_100a): tcgen05 + TMA + TMEM";
   m.def("forward_naive", &forward_naive, "Naive attention forward (CUDA-core baseline)",
@@ -264,4 +266,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("v"), py::arg("out"), py::arg("dout"), py::arg("lse"), py::arg("sm_scale") = 0.0,
         py::arg("is_causal") = false, py::arg("layout") = "bhnd");
   m.def("device_error", &device_error, "Read and clear kernel error flags (synchronises)");
+  bind_serving(m);
 }

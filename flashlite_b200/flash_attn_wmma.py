@@ -26,7 +26,30 @@ ring-attention steps; ``backward_flash2(q, k, v, out, dout, lse, sm_scale=0.0,
 is_causal=False) -> (dq, dk, dv)`` is the FA2 backward (head_dim 64; ``lse`` from
 ``forward_flash2_ex(..., return_lse=True)``, wrapped for autograd by
 ``flashlite_b200.attention.flash_attention``); ``device_error`` reads the
-error bits kernels raise when a bounded wait gives up.
+error bits kernels raise when a bounded wait gives up (bit 0) or an index is
+out of range (bit 1).
+
+Serving step and rotary positions (no reference counterpart; fp16 and bf16,
+rotary also fp32):
+
+* ``rotary(q, k, table, positions=None, interleaved=False, layout="bnhd",
+  out_q=None, out_k=None) -> (q, k)`` and its gradient ``rotary_backward(dq, dk,
+  table, positions=None, interleaved=False, layout="bnhd") -> (dq, dk)``; ``table``
+  from ``flashlite_b200.rotary.rotary_table``, wrapped for autograd by
+  ``flashlite_b200.rotary.rotary_embedding``.
+* ``plan_cache_step(context_lens, cu_seqlens, block_table, held_blocks, free_blocks,
+  num_free, total_tokens, page_size, parents=None, mask_words=0) -> (slots, positions,
+  admitted, num_free, held_blocks, tree_mask)`` gives new tokens their blocks, slots, positions
+  and, for trees of drafted tokens, ancestor masks, on the device.
+* ``rotary_append(q, k, v, table, positions, slots, k_cache, v_cache,
+  interleaved=False, layout="bnhd", out_q=None) -> q`` rotates q and k and writes k
+  and v to their slots.
+* ``tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_seqlens,
+  tree_mask=None, sm_scale=0.0, layout="bnhd", out=None, return_lse=False) -> (out,
+  lse)`` attends the new tokens to the paged cache; ``lse`` is ``[tokens, heads]``,
+  or None unless ``return_lse``.
+
+``flashlite_b200.serving.PagedCache`` holds the state these four calls share.
 """
 from __future__ import annotations
 
@@ -34,7 +57,8 @@ import torch  # noqa: F401  (loads libtorch/libc10 for the binding)
 
 try:
     from ._C import (backward_flash2, device_error, forward_block, forward_flash2,
-                     forward_flash2_ex, forward_naive, ring_finalize)
+                     forward_flash2_ex, forward_naive, plan_cache_step, ring_finalize, rotary,
+                     rotary_append, rotary_backward, tree_attention)
 except ImportError as exc:  # pragma: no cover - exercised only on unbuilt trees
     raise ImportError(
         "flashlite_b200 native extension is not built; run `python -m flashlite_b200.build` "
@@ -42,4 +66,5 @@ except ImportError as exc:  # pragma: no cover - exercised only on unbuilt trees
     ) from exc
 
 __all__ = ["forward_flash2", "forward_naive", "forward_flash2_ex", "forward_block", "ring_finalize",
-           "backward_flash2", "device_error"]
+           "backward_flash2", "device_error", "rotary", "rotary_backward", "rotary_append",
+           "plan_cache_step", "tree_attention"]

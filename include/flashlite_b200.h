@@ -31,7 +31,8 @@ typedef enum fl_status {
   FL_ERR_MISALIGNED = 3,       /* a pointer is not 16-byte aligned             */
   FL_ERR_CUDA = 4,             /* a CUDA runtime/driver call failed            */
   FL_ERR_NO_DEVICE = 5,        /* current device is not sm_100 (B200 class)    */
-  FL_ERR_DEVICE_TIMEOUT = 6    /* a kernel's bounded wait gave up (see below)  */
+  FL_ERR_DEVICE_TIMEOUT = 6,   /* a kernel's bounded wait gave up (see below)  */
+  FL_ERR_DEVICE_INDEX = 7      /* a kernel met an index out of range (below)   */
 } fl_status;
 
 /*
@@ -146,6 +147,137 @@ int fl_flash2_fwd_block_noalloc(const void* q, const void* k, const void* v, voi
                                 int64_t kv_offset, float sm_scale, int is_causal, int first,
                                 int last, void* stream);
 
+/* Element types of the serving and rotary entry points. */
+enum fl_dtype {
+  FL_DTYPE_F16 = 0,
+  FL_DTYPE_BF16 = 1,
+  FL_DTYPE_F32 = 2
+};
+
+/*
+ * Serving step and rotary positions; no reference counterpart (the reference
+ * has neither a cache nor positions). A paged cache is a pair of arrays of
+ * blocks of page_size rows; a request's row of the block table names its
+ * blocks in order, so that its cached token p lies in block
+ * table[p / page_size], row p % page_size: slot = block * page_size + row.
+ * Lengths, tables and slots live on the device and are read there, so no call
+ * waits for the GPU. An index that a kernel finds out of range is skipped
+ * and recorded: fl_device_error() then returns FL_ERR_DEVICE_INDEX.
+ * Strides count elements; the innermost dimension is contiguous.
+ */
+
+/*
+ * Rotary positions. q, k: [batch, length, heads, head_dim] by their strides
+ * {batch, token, head} (k may have other heads than q, or none). The first
+ * `rot` columns of each head turn in pairs, the others are copied: pair j is
+ * columns (j, j + rot/2), or (2j, 2j+1) if interleaved, and
+ * (x0, x1) -> (x0 c - x1 s, x1 c + x0 s), c = table[pos][j],
+ * s = table[pos][rot/2 + j] (fp32 rows of `rot` values). inverse != 0 negates
+ * s: the gradient with respect to the input. positions: int32 or int64, one
+ * per token (positions_batch != 0: [batch * length], else [length] for every
+ * batch entry); NULL means 0, 1, 2, ... A position outside the table gives
+ * NaN in the rotated columns. Outputs may be the inputs themselves.
+ * With slots != NULL ([batch * length] int64) the rotated k and the unchanged
+ * v go to row `slot` of k_out and v_out, caches of cache_blocks blocks of
+ * page_size rows with strides {block, row, head}; slot -1 writes nothing.
+ * Distinct tokens need distinct slots.
+ */
+typedef struct fl_rotary_args {
+  const void* q;
+  const void* k;
+  const void* v; /* cache form only */
+  void* q_out;
+  void* k_out;
+  void* v_out; /* cache form only */
+  const float* table;
+  const void* positions;
+  const int64_t* slots;
+  int64_t batch, length, heads, kv_heads, head_dim, rot, table_rows;
+  int64_t cache_blocks, page_size;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int64_t q_out_stride[3], k_out_stride[3], v_out_stride[3];
+  int32_t dtype, interleaved, inverse, positions_64, positions_batch;
+} fl_rotary_args;
+int fl_rotary(const fl_rotary_args* args, void* stream);
+
+/*
+ * Bookkeeping of one serving step. Request b has context_lens[b] cached
+ * tokens, held_blocks[b] blocks in its row of the table (at least those of its
+ * cached tokens; drafted tokens that were not kept leave more) and the new
+ * tokens cu_seqlens[b] .. cu_seqlens[b+1] - 1. Blocks that its new tokens need
+ * beyond those it holds are taken from the end of
+ * free_blocks[0 .. num_free[0] - 1], requests in order, and entered in its
+ * row of block_table (requests x table_cols, row stride table_stride), in
+ * place. A request whose blocks do not fit (its row, or what is free after
+ * the requests before it) is refused: admitted[b] = 0, its row unchanged,
+ * its slots -1. Out: slots and positions of the `tokens` new tokens (tokens
+ * past cu_seqlens[requests] get slot -1, position 0), admitted and
+ * held_after [requests], num_free_after [1].
+ * Trees: parents[t] is the index, within its request, of the token that t
+ * follows, smaller than its own, or -1 for the last cached token; the
+ * position of t is then context + depth, and tree_mask (tokens x mask_words
+ * 32-bit words, row-major) gets the bits of t and its ancestors. A request of
+ * a tree has at most 32 * mask_words tokens. parents NULL: each token follows
+ * the one before, position context + index, tree_mask unused.
+ * At most 16384 requests.
+ */
+typedef struct fl_plan_args {
+  const int32_t* context_lens;
+  const int32_t* cu_seqlens;
+  int32_t* block_table;
+  const int32_t* held_blocks;
+  const int32_t* free_blocks;
+  const int32_t* num_free;
+  const int32_t* parents;
+  int64_t* slots;
+  int32_t* positions;
+  uint8_t* admitted;
+  int32_t* held_after;
+  int32_t* num_free_after;
+  uint32_t* tree_mask;
+  int64_t requests, tokens, table_cols, table_stride, free_capacity, page_size, mask_words;
+} fl_plan_args;
+int fl_plan_cache_step(const fl_plan_args* args, void* stream);
+
+/*
+ * Attention of new tokens over a paged cache. Row t of q (tokens x heads x
+ * head_dim, strides {token, head}) is token i = t - cu_seqlens[b] of request
+ * b; it sees the context_lens[b] cached keys of its request and, of the
+ * request's own new tokens (already in the cache at context_lens[b] + i, see
+ * fl_rotary), those whose bit is set in its row of tree_mask (tokens x
+ * mask_words 32-bit words), or with tree_mask NULL those up to itself.
+ * heads is a multiple of kv_heads (at most 128 times): query head h reads key
+ * head h / (heads / kv_heads). k_cache, v_cache: num_blocks blocks of
+ * page_size rows, strides {block, row, head}; page_size is a power of two
+ * from 8 to 256; head_dim 64 or 128; fp16 or bf16. What lies in the cache
+ * outside the visible keys, NaN included, does not enter a row. out (tokens x
+ * heads x head_dim, contiguous); lse [tokens, heads] fp32 or NULL: natural-log
+ * log-sum-exp of the scaled scores. A row without a visible key gives 0 and
+ * -inf. sm_scale == 0 means 1/sqrt(head_dim). workspace: device memory of at
+ * least fl_tree_attention_workspace_size() bytes, 16-byte aligned, for this
+ * call alone until it has run. At most 4096 requests.
+ */
+typedef struct fl_tree_attention_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* out;
+  float* lse;
+  const int32_t* block_table;
+  const int32_t* context_lens;
+  const int32_t* cu_seqlens;
+  const uint32_t* tree_mask;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t tokens, requests, heads, kv_heads, head_dim;
+  int64_t num_blocks, page_size, table_cols, table_stride, mask_words;
+  int64_t q_stride[2], k_stride[3], v_stride[3];
+  int32_t dtype;
+  float sm_scale;
+} fl_tree_attention_args;
+size_t fl_tree_attention_workspace_size(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim);
+int fl_tree_attention(const fl_tree_attention_args* args, void* stream);
+
 /* Human-readable text for a status code (static storage). */
 const char* fl_status_str(int status);
 
@@ -155,7 +287,8 @@ const char* fl_last_error(void);
 /*
  * Reads and clears the device error word of the current device after
  * synchronising `stream`. Writes the raw bit flags to *flags (may be NULL)
- * and returns FL_ERR_DEVICE_TIMEOUT if any kernel gave up a wait, else FL_OK.
+ * and returns FL_ERR_DEVICE_TIMEOUT if any kernel gave up a wait (bit 0), else
+ * FL_ERR_DEVICE_INDEX if one met an index out of range (bit 1), else FL_OK.
  */
 int fl_device_error(void* stream, uint32_t* flags);
 
