@@ -35,10 +35,10 @@ int guarded(Body&& body) noexcept {
 // the previous one on the stream drains, and waits for its results itself
 // (griddepcontrol.wait before the first access to global memory).
 template <typename Params>
-cudaError_t launch_pdl(void (*kern)(Params), int blocks, int threads, int smem, cudaStream_t stream,
+cudaError_t launch_pdl(void (*kern)(Params), dim3 blocks, int threads, int smem, cudaStream_t stream,
                        const Params& prm) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
+  cfg.gridDim = blocks;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

@@ -304,12 +304,12 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
       : "memory");
 }
 
-// Instruction descriptor, .kind::f16, fp16 A/B, fp32 accumulator, dense.
-//   bits 4-5 D format (1 = F32), 7-9 A format (0 = F16), 10-12 B format,
+// Instruction descriptor, .kind::f16, fp16 (or bf16) A/B, fp32 accumulator, dense.
+//   bits 4-5 D format (1 = F32), 7-9 A format (0 = F16, 1 = BF16), 10-12 B format (the same),
 //   15 A major (0 = K), 16 B major (0 = K, 1 = MN), 17-22 N>>3, 24-28 M>>4.
 __host__ __device__ constexpr uint32_t make_idesc_f16_f32(int M, int N, bool b_mn_major,
-                                                          bool a_mn_major = false) {
-  return (1u << 4) | (0u << 7) | (0u << 10) | ((a_mn_major ? 1u : 0u) << 15) |
+                                                          bool a_mn_major = false, bool bf16 = false) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn_major ? 1u : 0u) << 15) |
          ((b_mn_major ? 1u : 0u) << 16) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
@@ -526,6 +526,13 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// The same as bf16x2.
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 

@@ -1,15 +1,41 @@
 // Attention of new tokens (one, a chunk, or a tree of drafted ones) over a
-// paged cache: the plain kernel, one warp per (token, query head).
+// paged cache, on the tensor cores.
 //
-//   o_t = sum_j w_tj v_j / l_t,  w_tj = exp(scale q_t.k_j - m_t),
-//   m_t = max_j, l_t = sum_j w_tj over the keys j that t sees:
-//   the cached ones and the new ones its mask (or the causal rule) names.
+//   o_t = sum_j w_tj v_j / l_t,  w_tj = 2^(scale log2(e) q_t.k_j - m_t),
+//   l_t = sum_j w_tj, over the keys j that token t sees: the cached ones and
+//   the new ones that its mask (or the causal rule) names. m_t is a running
+//   reference maximum; a row that sees nothing gives 0 and -inf.
+//
+// A unit of work is (request, key head, row tile): up to 128 rows, the
+// request's tokens times the query heads that share the key head, so that
+// each key and value is read once for all of them. Rows that a short request
+// leaves empty cost nothing in the memory-bound case: the tensor cores finish
+// a 128-row product in a fraction of the time its keys take to arrive, and
+// softmax warps without rows skip it. A unit's keys are cut into tiles (kBN
+// keys, gathered page by page with TMA); all tiles of all units, laid end to
+// end, are divided evenly among the CTAs whatever the requests' lengths, which
+// the kernel reads on the device. A CTA that ends up with part of a unit
+// leaves an fp32 partial result, and a second kernel joins the parts of each
+// cut unit in order (no atomics: the same bits every time).
+//
+// A CTA is a scheduler warp, K and V producer warps, an MMA warp and one
+// softmax warpgroup, one thread per row; two CTAs share an SM and fill each
+// other's waits. S and O accumulate in TMEM, P goes to TMEM as operand A.
+//
+// Keys that no row may see are kept out of the products as zeros: masked
+// scores are replaced, not added to, and V rows past the visible keys are
+// cleared in shared memory, since 0 times what an unused row holds may be
+// NaN. Rows of V that some rows see and others do not are searched for
+// infinities and NaN, which are cleared too and added back, in the epilogue,
+// to the rows that see them.
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -21,76 +47,877 @@ namespace fl {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBM = 128;           // rows per unit (UMMA M)
 constexpr int kMaxRequests = 4096;
+constexpr uint32_t kTmemCols = 256;
+constexpr int kSegRing = 4;        // work descriptors between the scheduler and the other warps
+constexpr int kSegReaders = 7;     // K, V, MMA and four softmax warps
+constexpr int kCtasPerSm = 2;
+// Fewest tiles worth a CTA of their own.
+#ifndef FL_TREE_MIN_STEPS
+#define FL_TREE_MIN_STEPS 1
+#endif
+
+// Shape per head dimension; tiles are made of 64-column (128-byte) swizzle
+// atoms as in the other forward kernels. K and V tiles are 16 KB both ways;
+// two CTAs share an SM's 228 KB.
+//   TMEM columns: S (kBN) | O (HD) | P (kBN / 2): 256 and 224.
+template <int HD>
+struct Shape {
+  static_assert(HD == 64 || HD == 128, "head dimension 64 or 128");
+  static constexpr int kBN = HD == 64 ? 128 : 64;
+  static constexpr int kHalves = HD / 64;
+  static constexpr int kStagesK = 3;
+  static constexpr int kStagesV = HD == 64 ? 3 : 2;
+  static constexpr int kQBytes = kBM * HD * 2;
+  static constexpr int kTileBytes = kBN * HD * 2;
+  static constexpr int kSmemQ = 0;
+  static constexpr int kSmemK = kSmemQ + kQBytes;
+  static constexpr int kSmemV = kSmemK + kStagesK * kTileBytes;
+  static constexpr int kSmemMisc = kSmemV + kStagesV * kTileBytes;
+  static constexpr int kSmemBytes = kSmemMisc + 1024;
+  static constexpr uint32_t kColS = 0, kColO = kBN, kColP = kBN + HD;
+  static_assert(kColP + kBN / 2 <= kTmemCols, "TMEM");
+  static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
+};
+// Register split: 128 x 64 (producers, MMA, scheduler) + 128 x 192 (softmax) = 256 x 128, the launch's total.
+constexpr int kRegsProducer = 64, kRegsSoftmax = 192;
+
+// A reference maximum is kept until a row's maximum exceeds it by this much
+// (log2); probabilities are held 2^kUp times their size, so that fp16 keeps
+// the small ones out of its subnormal range: at most 2^15 after the lag.
+constexpr float kLag = 8.0f, kUp = 7.0f;
 
 struct TreeParams {
-  fl_tree_attention_args a;
-  float scale_log2;
-  int page_shift;
+  CUtensorMap tm_q;  // {D, heads, tokens}, box {64, group, tokens per row tile}
+  CUtensorMap tm_k;  // {D, page rows, key heads, blocks}, box {64, min(page, kBN), 1, 1}
+  CUtensorMap tm_v;
+  const void* v;
+  void* out;
+  float* lse;
+  const int32_t* table;
+  const int32_t* context;
+  const int32_t* cu;
+  const uint32_t* mask;
+  float* part;       // [2 * grid][128][D] fp32, then [2 * grid][128] log2-sum-exp
+  float* part_lse;
+  int4* cuts;        // [grid]: parts after the first, first token, head and rows of the cut unit that starts there
   unsigned int* err;
+  long long v_stride[3];
+  long long table_stride;
+  int requests, tokens, heads, kv_heads, group, tile_tokens;
+  int page_shift, box_rows, num_blocks, table_cols, mask_words;
+  float scale_log2;
+  int grid;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_constant__ TreeParams p) {
-  const fl_tree_attention_args& a = p.a;
+// One request as the schedule sees it.
+struct Request {
+  int begin, count, ctx, room;  // first row of q, new tokens, cached tokens, keys its table row can name
+};
+
+__device__ __forceinline__ Request request_of(const TreeParams& p, int begin, int end, int ctx, bool report) {
+  Request r;
+  const long long room = static_cast<long long>(p.table_cols) << p.page_shift;
+  r.room = room > 0x3fffffff ? 0x3fffffff : static_cast<int>(room);
+  bool sound = true;
+  r.begin = begin;
+  r.count = end - begin;
+  if (begin < 0 || end < begin || end > p.tokens) {
+    sound = false;
+    r.begin = r.count = 0;
+  }
+  r.ctx = ctx;
+  if (ctx < 0 || ctx > r.room) {
+    sound = false;
+    r.ctx = ctx < 0 ? 0 : r.room;
+  }
+  if (r.count > r.room - r.ctx) sound = false;  // the new tokens past the table's end are not visible
+  if (!sound && report) atomicOr(p.err, kDevErrIndex);
+  return r;
+}
+
+// Keys that some row of the row tile with tokens [i0, i0 + n) may see.
+__device__ __forceinline__ int keys_of(const TreeParams& p, const Request& r, int i0) {
+  int inner;
+  if (p.mask != nullptr) inner = min(r.count, 32 * p.mask_words);
+  else inner = min(r.count, i0 + p.tile_tokens);
+  return min(r.ctx + inner, r.room);
+}
+
+template <int kBN>
+__device__ __forceinline__ int tiles_of(const TreeParams& p, const Request& r, int i0) {
+  return max(1, (keys_of(p, r, i0) + kBN - 1) / kBN);
+}
+
+// Tiles of one key head of a request: those of all its row tiles.
+template <int kBN>
+__device__ __forceinline__ long long head_tiles(const TreeParams& p, const Request& r) {
+  if (r.count == 0) return 0;
+  if (p.mask != nullptr)
+    return static_cast<long long>((r.count + p.tile_tokens - 1) / p.tile_tokens) * tiles_of<kBN>(p, r, 0);
+  long long n = 0;
+  for (int i0 = 0; i0 < r.count; i0 += p.tile_tokens) n += tiles_of<kBN>(p, r, i0);
+  return n;
+}
+
+// A CTA's share of one unit: tiles [t0, t1) of n.
+struct Segment {
+  int request, head, i0, rows;  // rows = tokens in the row tile times group
+  int begin, count, ctx, keys;
+  int t0, t1;                   // t1 < 0: no more work
+  int slot;                     // partial result, -1: the whole unit, written to out
+  int pad;
+};
+
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err));
+}
+__device__ __forceinline__ bool wait_all_issuer(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                                unsigned int* err) {
+  return __all_sync(0xffffffffu, mbar_wait_issuer(bar, parity, abort_flag, err));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+
+// Exponent bits of the type, all set in infinities and NaN.
+template <typename T>
+constexpr uint32_t kExpBits = 0x7C00u;
+template <>
+constexpr uint32_t kExpBits<__nv_bfloat16> = 0x7F80u;
+
+// A pair with its infinite and NaN elements cleared.
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  constexpr uint32_t e = kExpBits<T>;
+  if ((w & e) == e) w &= 0xffff0000u;
+  if ((w >> 16 & e) == e) w &= 0x0000ffffu;
+  return w;
+}
+
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Makes a V tile safe for the product, by one warp: rows [valid, kBN) cleared,
+// infinities and NaN in rows [mixed, valid) cleared. Returns whether any were.
+template <typename T, int HD>
+__device__ __forceinline__ bool guard_v(uint32_t tile, int mixed, int valid, int lane) {
+  constexpr int kBN = Shape<HD>::kBN;
+  bool bad = false;
+#pragma unroll
+  for (int hh = 0; hh < Shape<HD>::kHalves; ++hh) {
+    const uint32_t half = tile + hh * (kBN * 128);
+    for (int c = valid * 8 + lane; c < kBN * 8; c += 32) st_shared_v4(half + c * 16, 0u, 0u, 0u, 0u);
+    for (int c = mixed * 8 + lane; c < valid * 8; c += 32) {
+      const uint4 v = ld_shared_v4(half + c * 16);
+      const uint4 f = make_uint4(finite2<T>(v.x), finite2<T>(v.y), finite2<T>(v.z), finite2<T>(v.w));
+      if (f.x != v.x || f.y != v.y || f.z != v.z || f.w != v.w) {
+        st_shared_v4(half + c * 16, f.x, f.y, f.z, f.w);
+        bad = true;
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  return __any_sync(0xffffffffu, bad);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(const __grid_constant__ TreeParams p) {
+  using C = Shape<HD>;
+  constexpr int kBN = C::kBN;
+  constexpr int kStagesK = C::kStagesK, kStagesV = C::kStagesV;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t s_q = sbase + C::kSmemQ, s_k0 = sbase + C::kSmemK, s_v0 = sbase + C::kSmemV;
+  // misc block: barriers | segments | scan scratch | flags
+  const uint32_t bars = sbase + C::kSmemMisc;
+  const uint32_t bar_kfull = bars, bar_kempty = bar_kfull + 8 * kStagesK;
+  const uint32_t bar_vfull = bar_kempty + 8 * kStagesK, bar_vempty = bar_vfull + 8 * kStagesV;
+  const uint32_t bar_segfull = bar_vempty + 8 * kStagesV, bar_segempty = bar_segfull + 8 * kSegRing;
+  const uint32_t bar_x = bar_segempty + 8 * kSegRing;
+  const uint32_t bar_qfull = bar_x, bar_qfree = bar_x + 8, bar_s = bar_x + 16, bar_sfree = bar_x + 24, bar_p = bar_x + 32,
+                 bar_pv = bar_x + 40, bar_ofree = bar_x + 48, bar_seg = bar_x + 56, bar_drain = bar_x + 64;
+  constexpr int kBarBytes = 8 * (2 * kStagesK + 2 * kStagesV + 2 * kSegRing + 9);
+  constexpr int kSegOff = (kBarBytes + 15) / 16 * 16;
+  uint8_t* misc = smem + C::kSmemMisc;
+  Segment* segs = reinterpret_cast<Segment*>(misc + kSegOff);
+  constexpr int kScanOff = kSegOff + kSegRing * static_cast<int>(sizeof(Segment));
+  long long* s_scan = reinterpret_cast<long long*>(misc + kScanOff);  // one per warp
+  struct Start {
+    long long offset, total, s0, s1;
+    int request, used;
+  };
+  Start* start = reinterpret_cast<Start*>(misc + kScanOff + 8 * (kThreads / 32));
+  constexpr int kFlagOff = kScanOff + 8 * (kThreads / 32) + static_cast<int>(sizeof(Start));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + kFlagOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + kFlagOff + 4);
+  volatile int* bad_flag = reinterpret_cast<volatile int*>(misc + kFlagOff + 8);
+  static_assert(kFlagOff + 16 <= 1024, "misc block");
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x;
+
+  // ---- setup ----
+  if (tid == 0) {
+    for (int st = 0; st < kStagesK; ++st) {
+      mbar_init(bar_kfull + 8 * st, 1);
+      mbar_init(bar_kempty + 8 * st, 1);
+    }
+    for (int st = 0; st < kStagesV; ++st) {
+      mbar_init(bar_vfull + 8 * st, 1);
+      mbar_init(bar_vempty + 8 * st, 1);
+    }
+    for (int st = 0; st < kSegRing; ++st) {
+      mbar_init(bar_segfull + 8 * st, 1);
+      mbar_init(bar_segempty + 8 * st, kSegReaders);
+    }
+    mbar_init(bar_qfull, 1);
+    mbar_init(bar_qfree, 1);
+    mbar_init(bar_s, 1);
+    mbar_init(bar_sfree, 4);  // one arrival per softmax warp
+    mbar_init(bar_p, 4);
+    mbar_init(bar_pv, 1);
+    mbar_init(bar_ofree, 4);
+    mbar_init(bar_seg, 1);
+    mbar_init(bar_drain, 1);
+    *abort_flag = 0;
+    *bad_flag = 0;
+    start->request = -1;
+    fence_mbar_init();
+    tma_prefetch_desc(&p.tm_q);
+    tma_prefetch_desc(&p.tm_k);
+    tma_prefetch_desc(&p.tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- this CTA's share: prefix sum of the requests' tiles ----
+  {
+    const int per = (p.requests + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, p.requests), b1 = min(b0 + per, p.requests);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b)
+      mine += p.kv_heads * head_tiles<kBN>(p, request_of(p, p.cu[b], p.cu[b + 1], p.context[b], cta == 0));
+    long long incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += x;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const long long x = s_scan[w];
+      if (w < warp) before += x;
+      total += x;
+    }
+    before += incl - mine;
+    const long long most = (total + FL_TREE_MIN_STEPS - 1) / FL_TREE_MIN_STEPS;
+    const int used = static_cast<int>(min(static_cast<long long>(p.grid), most));
+    const long long s0 = cta < used ? cta * total / used : 0, s1 = cta < used ? (cta + 1) * total / used : 0;
+    if (s0 < s1 && before <= s0 && s0 < before + mine) {
+      long long at = before;
+      for (int b = b0; b < b1; ++b) {
+        const long long n = p.kv_heads * head_tiles<kBN>(p, request_of(p, p.cu[b], p.cu[b + 1], p.context[b], false));
+        if (s0 < at + n) {
+          start->request = b;
+          start->offset = s0 - at;
+          break;
+        }
+        at += n;
+      }
+    }
+    if (tid == 0) {
+      start->total = total;
+      start->used = used;
+      start->s0 = s0;
+      start->s1 = s1;
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsProducer));
+    if (warp == 3) {
+      // ======================= scheduler =======================
+      const long long total = start->total;
+      const int used = start->used;
+      long long s = start->s0;
+      const long long s1 = start->s1;
+      int b = start->request;
+      long long off = b >= 0 ? start->offset : 0;
+      int ring = 0;
+      bool ok = true;
+      int4 cut = make_int4(0, 0, 0, 0);  // x: parts after the first (0: no unit is cut here)
+      auto post = [&](const Segment& g) -> bool {
+        const int st = ring % kSegRing;
+        if (!wait_all(bar_segempty + 8 * st, ((ring / kSegRing) & 1) ^ 1, abort_flag, p.err)) return false;
+        if (lane == 0) {
+          segs[st] = g;
+          mbar_arrive(bar_segfull + 8 * st);
+        }
+        __syncwarp();
+        ++ring;
+        return true;
+      };
+      int base = -64;  // lane l holds request base + l
+      int l_begin = 0, l_end = 0, l_ctx = 0;
+      while (ok && s < s1 && b >= 0 && b < p.requests) {
+        if (b >= base + 32 || b < base) {
+          base = b;
+          const int mine = b + lane;
+          l_begin = mine < p.requests ? p.cu[mine] : 0;
+          l_end = mine < p.requests ? p.cu[mine + 1] : 0;
+          l_ctx = mine < p.requests ? p.context[mine] : 0;
+        }
+        const Request r = request_of(p, __shfl_sync(0xffffffffu, l_begin, b - base),
+                                     __shfl_sync(0xffffffffu, l_end, b - base),
+                                     __shfl_sync(0xffffffffu, l_ctx, b - base), false);
+        int h = 0, i0 = 0;
+        if (off > 0) {  // the first request starts part-way
+          const long long per_head = head_tiles<kBN>(p, r);
+          h = static_cast<int>(off / per_head);
+          off -= h * per_head;
+          while (off >= tiles_of<kBN>(p, r, i0)) {
+            off -= tiles_of<kBN>(p, r, i0);
+            i0 += p.tile_tokens;
+          }
+        }
+        for (; ok && s < s1 && r.count > 0 && h < p.kv_heads; ++h, i0 = 0) {
+          for (; ok && s < s1 && i0 < r.count; i0 += p.tile_tokens) {
+            const int n = tiles_of<kBN>(p, r, i0);
+            Segment g;
+            g.request = b;
+            g.head = h;
+            g.i0 = i0;
+            g.rows = min(p.tile_tokens, r.count - i0) * p.group;
+            g.begin = r.begin;
+            g.count = r.count;
+            g.ctx = r.ctx;
+            g.keys = keys_of(p, r, i0);
+            g.t0 = static_cast<int>(off);
+            g.t1 = static_cast<int>(min(static_cast<long long>(n), off + (s1 - s)));
+            const bool whole = g.t0 == 0 && g.t1 == n;
+            g.slot = whole ? -1 : 2 * cta + (g.t0 == 0 ? 1 : 0);
+            g.pad = 0;
+            if (!whole && g.t0 == 0) {
+              // the unit's first part: the last CTA with tiles of it
+              const long long end = s + n;
+              const int last = static_cast<int>((end * used + total - 1) / total) - 1;
+              cut = make_int4(last - cta, r.begin + i0, h, g.rows);
+            }
+            s += g.t1 - g.t0;
+            off = 0;
+            ok = post(g);
+          }
+        }
+        ++b;
+        off = 0;
+      }
+      if (ok) {
+        Segment g = {};
+        g.t1 = -1;
+        post(g);
+      }
+      if (lane == 0) p.cuts[cta] = cut;
+    } else if (warp == 0 || warp == 2) {
+      // ======================= K (and Q) producer, V producer =======================
+      const bool is_k = warp == 0;
+      const int stages = is_k ? kStagesK : kStagesV;
+      const CUtensorMap* tm = is_k ? &p.tm_k : &p.tm_v;
+      const uint32_t ring0 = is_k ? s_k0 : s_v0, full0 = is_k ? bar_kfull : bar_vfull, empty0 = is_k ? bar_kempty : bar_vempty;
+      const int page = 1 << p.page_shift;
+      const int boxes = kBN / p.box_rows;  // page boxes per tile
+      int tile = 0, seg = 0, q_loads = 0;
+      bool ok = true;
+      while (ok) {
+        const int sl = seg % kSegRing;
+        if (!wait_all(bar_segfull + 8 * sl, (seg / kSegRing) & 1, abort_flag, p.err)) break;
+        const Segment g = segs[sl];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_segempty + 8 * sl);
+        ++seg;
+        if (g.t1 < 0) break;
+        const int32_t* row = p.table + g.request * p.table_stride;
+        // this lane's box of tile t: its block and first row there
+        auto block_of = [&](int t) -> int {
+          const int key = t * kBN + lane * p.box_rows;
+          if (lane >= boxes || key >= g.keys) return -1;
+          const int blk = row[key >> p.page_shift];
+          if (blk >= 0 && blk < p.num_blocks) return blk;
+          if (is_k) atomicOr(p.err, kDevErrIndex);
+          return p.num_blocks;  // outside the map: zeros arrive, nothing is read
+        };
+        int next = block_of(g.t0);
+        if (is_k) {
+          if (!wait_all(bar_qfree, (q_loads & 1) ^ 1, abort_flag, p.err)) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar_qfull, p.group * p.tile_tokens * 128 * C::kHalves);
+#pragma unroll
+            for (int hh = 0; hh < C::kHalves; ++hh)
+              tma_load_3d(s_q + hh * (kBM * 128), &p.tm_q, bar_qfull, 64 * hh, g.head * p.group, g.begin + g.i0);
+          }
+          __syncwarp();
+          ++q_loads;
+        }
+        for (int t = g.t0; t < g.t1; ++t, ++tile) {
+          const int blk = next;
+          if (t + 1 < g.t1) next = block_of(t + 1);
+          const int st = tile % stages;
+          if (!wait_all(empty0 + 8 * st, ((tile / stages) & 1) ^ 1, abort_flag, p.err)) {
+            ok = false;
+            break;
+          }
+          const int live = __popc(__ballot_sync(0xffffffffu, blk >= 0));
+          if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, live * p.box_rows * 128 * C::kHalves);
+          __syncwarp();
+          if (blk >= 0) {
+            const int key = t * kBN + lane * p.box_rows;
+#pragma unroll
+            for (int hh = 0; hh < C::kHalves; ++hh)
+              tma_load_4d(ring0 + st * C::kTileBytes + hh * (kBN * 128) + lane * p.box_rows * 128, tm, full0 + 8 * st,
+                          64 * hh, key & (page - 1), g.head, blk);
+          }
+          __syncwarp();
+        }
+      }
+      if (*abort_flag && lane == 0) {
+        // let every copy this warp started land before shared memory is released
+        for (int t = tile > stages ? tile - stages : 0; t < tile; ++t)
+          mbar_wait_quiet(full0 + 8 * (t % stages), (t / stages) & 1);
+        if (is_k && q_loads > 0) mbar_wait_quiet(bar_qfull, (q_loads - 1) & 1);
+      }
+    } else {
+      // ======================= MMA issuer =======================
+      constexpr uint32_t idesc_s = make_idesc_f16_f32(kBM, kBN, false, false, kBf16);
+      constexpr uint32_t idesc_pv = make_idesc_f16_f32(kBM, HD, true, false, kBf16);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t dq = make_sdesc_sw128(s_q, 16, 1024);
+      const uint64_t dk0 = make_sdesc_sw128(s_k0, 16, 1024);
+      const uint64_t dv0 = make_sdesc_sw128(s_v0, HD == 64 ? 8192 : kBN * 128, 1024);
+      constexpr uint64_t kStageEnc = C::kTileBytes >> 4, kQHalf = (kBM * 128) >> 4, kKHalf = (kBN * 128) >> 4;
+      int ks = 0, vs = 0, seg = 0;  // S products, P V products, segments so far
+      bool ok = true;
+      while (ok) {
+        const int sl = seg % kSegRing;
+        if (!wait_all_issuer(bar_segfull + 8 * sl, (seg / kSegRing) & 1, abort_flag, p.err)) break;
+        const Segment g = segs[sl];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_segempty + 8 * sl);
+        if (g.t1 < 0) break;
+        if (!wait_all_issuer(bar_qfull, seg & 1, abort_flag, p.err)) break;
+        auto issue_s = [&](bool last) -> bool {
+          const int st = ks % kStagesK;
+          if (!wait_all_issuer(bar_kfull + 8 * st, (ks / kStagesK) & 1, abort_flag, p.err)) return false;
+          if (!wait_all_issuer(bar_sfree, (ks & 1) ^ 1, abort_flag, p.err)) return false;
+          tc_fence_after();
+          const uint64_t bd = dk0 + st * kStageEnc;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+              umma_f16_ss(tm + C::kColS, dq + 2 * (kk & 3) + (kk >> 2) * kQHalf, bd + 2 * (kk & 3) + (kk >> 2) * kKHalf,
+                          idesc_s, kk > 0 ? 1u : 0u);
+            umma_commit(bar_s);
+            umma_commit(bar_kempty + 8 * st);
+            if (last) umma_commit(bar_qfree);
+          }
+          __syncwarp();
+          ++ks;
+          return true;
+        };
+        ok = issue_s(g.t0 + 1 == g.t1);
+        // O of the segment before has been read
+        if (ok) ok = wait_all_issuer(bar_ofree, (seg & 1) ^ 1, abort_flag, p.err);
+        if (!ok) break;
+        if (lane == 0) *bad_flag = 0;
+        // keys from here on are hidden from some row of the tile
+        const int mixed = p.mask != nullptr ? g.ctx : min(g.ctx + g.i0 + 1, g.keys);
+        for (int t = g.t0; t < g.t1; ++t) {
+          if (t + 1 < g.t1 && !(ok = issue_s(t + 2 == g.t1))) break;
+          const int st = vs % kStagesV;
+          if (!(ok = wait_all_issuer(bar_vfull + 8 * st, (vs / kStagesV) & 1, abort_flag, p.err))) break;
+          const int valid = min(kBN, g.keys - t * kBN), from = max(0, min(mixed - t * kBN, valid));
+          if (from < kBN) {
+            const bool bad = guard_v<T, HD>(s_v0 + st * C::kTileBytes, from, valid, lane);
+            if (bad && lane == 0) *bad_flag = 1;
+            __syncwarp();
+          }
+          if (!(ok = wait_all_issuer(bar_p, vs & 1, abort_flag, p.err))) break;
+          tc_fence_after();
+          const uint64_t bd = dv0 + st * kStageEnc;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kBN / 16; ++kk)
+              umma_f16_ts(tm + C::kColO, tm + C::kColP + kk * 8, bd + 128 * kk, idesc_pv,
+                          (kk > 0 || t > g.t0) ? 1u : 0u);
+            umma_commit(bar_pv);
+            umma_commit(bar_vempty + 8 * st);
+          }
+          __syncwarp();
+          ++vs;
+        }
+        if (lane == 0) mbar_arrive(bar_seg);  // publishes bad_flag
+        __syncwarp();
+        ++seg;
+      }
+      // wait until every MMA this warp issued has completed
+      if (elect_one()) {
+        umma_commit(bar_drain);
+        mbar_wait_quiet(bar_drain, 0);
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsSoftmax));
+    // ======================= softmax: one thread per row =======================
+    const int t_row = tid - 128;
+    const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t tS = tmem + lane_base + C::kColS, tP = tmem + lane_base + C::kColP, tO = tmem + lane_base + C::kColO;
+    const int my_token = t_row / p.group, my_head = t_row % p.group;  // within the row tile
+    const float sc = p.scale_log2;
+    const bool prescale = !(sc > 0.0f);  // a negative scale turns maxima into minima: applied first
+    int js = 0, seg = 0;                 // tiles and segments so far
+    bool ok = true;
+    while (ok) {
+      const int sl = seg % kSegRing;
+      if (!wait_all(bar_segfull + 8 * sl, (seg / kSegRing) & 1, abort_flag, p.err)) break;
+      const Segment g = segs[sl];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_segempty + 8 * sl);
+      if (g.t1 < 0) break;
+      const bool live_warp = 32 * (warp & 3) < g.rows;  // warps without rows only keep the barriers going
+      const bool live = t_row < g.rows;
+      const int token = g.begin + g.i0 + my_token;      // row of q, if live
+      // keys this row sees without looking at its mask, and where its mask ends
+      const int plain = p.mask != nullptr ? min(g.ctx, g.keys) : min(g.ctx + g.i0 + my_token + 1, g.keys);
+      const uint32_t* words = p.mask != nullptr && live ? p.mask + static_cast<long long>(token) * p.mask_words : nullptr;
+      float m_ref = -INFINITY, l = 0.0f, l_fix = 0.0f;
+      for (int t = g.t0; t < g.t1; ++t, ++js) {
+        if (!(ok = wait_all(bar_s, js & 1, abort_flag, p.err))) break;
+        if (!live_warp) {
+          if (lane == 0) mbar_arrive(bar_sfree);
+          if (t > g.t0 && !(ok = wait_all(bar_pv, (js - 1) & 1, abort_flag, p.err))) break;
+          if (lane == 0) mbar_arrive(bar_p);
+          continue;
+        }
+        tc_fence_after();
+        uint32_t sr[kBN];
+        if constexpr (kBN == 128) tmem_ld128_wait(tS, sr);
+        else tmem_ld64_wait(tS, sr);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_sfree);
+        float s[kBN];
+#pragma unroll
+        for (int c = 0; c < kBN; ++c) s[c] = __uint_as_float(sr[c]);
+        float scl = sc;
+        if (prescale) {
+#pragma unroll
+          for (int c = 0; c < kBN; ++c) s[c] *= sc;
+          scl = 1.0f;
+        }
+        const int k0 = t * kBN;
+        if (__any_sync(0xffffffffu, plain < k0 + kBN)) {
+#pragma unroll
+          for (int q = 0; q < kBN / 32; ++q) {
+            // bit c: column 32 q + c is visible
+            const int first = plain - (k0 + 32 * q);
+            uint32_t vis = first <= 0 ? 0u : first >= 32 ? 0xffffffffu : (1u << first) - 1u;
+            if (words != nullptr && first < 32) {
+              const int j0 = k0 + 32 * q - g.ctx;  // new token of column 0; may be negative
+              const int w = j0 >> 5, sh = j0 & 31;
+              const uint32_t lo = w >= 0 && w < p.mask_words ? words[w] : 0u;
+              const uint32_t hi = w + 1 >= 0 && w + 1 < p.mask_words ? words[w + 1] : 0u;
+              uint32_t bits = __funnelshift_r(lo, hi, sh);
+              const int end = g.keys - (k0 + 32 * q);
+              if (end < 32) bits &= end <= 0 ? 0u : (1u << end) - 1u;
+              vis |= bits;
+            }
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[32 * q + c] = (vis >> c & 1u) ? s[32 * q + c] : -INFINITY;
+          }
+        }
+        float mx;
+        {
+          float part[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            constexpr int L = kBN / 4;
+            float a = fmaxf(s[q * L], s[q * L + 1]);
+#pragma unroll
+            for (int e = 2; e < L; e += 2) a = fmax3(a, s[q * L + e], s[q * L + e + 1]);
+            part[q] = a;
+          }
+          mx = fmax3(fmaxf(part[0], part[1]), part[2], part[3]);
+        }
+        // The argument of 2^x is one fused multiply-add, exact up to its own
+        // rounding, while the reference is a rounded product: past 2^20 that
+        // rounding alone could empty a row, and scores are scaled first.
+        const float mag = fabsf(mx * scl);
+        if (__any_sync(0xffffffffu, mag > 1048576.0f && mag < INFINITY) && !prescale) {
+#pragma unroll
+          for (int c = 0; c < kBN; ++c) s[c] *= sc;
+          mx *= sc;
+          scl = 1.0f;
+        }
+        const float m_new = fmaxf(m_ref, mx * scl);
+        const bool need = m_new > m_ref + kLag;
+        float alpha = 1.0f;
+        if (need) {
+          alpha = ex2_approx(m_ref - m_new);
+          m_ref = m_new;
+        }
+        l *= alpha;
+        l_fix *= alpha;
+        const float m_use = (m_ref == -INFINITY) ? 0.0f : m_ref - kUp;
+        const float2 scl2 = make_float2(scl, scl), nm2 = make_float2(-m_use, -m_use);
+        float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t pk[kBN / 2];
+#pragma unroll
+        for (int e = 0; e < kBN / 2; ++e) {
+          const float2 x = __ffma2_rn(make_float2(s[2 * e], s[2 * e + 1]), scl2, nm2);
+          const float2 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          sum[e & 3] = __fadd2_rn(sum[e & 3], pp);
+          pk[e] = pack2<T>(pp.x, pp.y);
+        }
+        {
+          const float2 a = __fadd2_rn(sum[0], sum[1]), b = __fadd2_rn(sum[2], sum[3]);
+          l += (a.x + a.y) + (b.x + b.y);
+          // The tile's largest p enters O rounded: O's normaliser sees the
+          // same value, so that a row which one key dominates gives that
+          // key's value exactly; the log-sum-exp keeps the unrounded sum.
+          const float pm = ex2_approx(fmaf(mx, scl, -m_use));
+          l_fix += static_cast<float>(static_cast<T>(pm)) - pm;
+        }
+        // P V of the tile before: its P is free to be overwritten, O to be rescaled
+        if (t > g.t0) {
+          if (!(ok = wait_all(bar_pv, (js - 1) & 1, abort_flag, p.err))) break;
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, need)) {
+            uint32_t o[32];
+#pragma unroll
+            for (int h = 0; h < HD / 32; ++h) {
+              tmem_ld32_wait(tO + h * 32, o);
+#pragma unroll
+              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+              tmem_st32(tO + h * 32, o);
+            }
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < kBN / 32; ++q)
+          tmem_st16(tP + q * 16, *reinterpret_cast<const uint32_t(*)[16]>(&pk[q * 16]));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p);
+      }
+      if (!ok) break;
+
+      // ---- epilogue of the segment ----
+      if (!(ok = wait_all(bar_pv, (js - 1) & 1, abort_flag, p.err))) break;
+      if (!(ok = wait_all(bar_seg, seg & 1, abort_flag, p.err))) break;
+      tc_fence_after();
+      if (live_warp) {
+        const bool bad = *bad_flag != 0;
+        const float norm = l + l_fix;
+        const float inv = (l > 0.0f) ? 1.0f / norm : 0.0f;
+        const float lse2 = (l == 0.0f) ? -INFINITY : (m_ref - kUp) + log2f(l);
+        const long long orow = static_cast<long long>(token) * p.heads + g.head * p.group + my_head;
+        float* prow = g.slot < 0 ? nullptr : p.part + (static_cast<long long>(g.slot) * kBM + t_row) * HD;
+        if (live) {
+          if (g.slot >= 0) p.part_lse[g.slot * kBM + t_row] = lse2;
+          else if (p.lse != nullptr) p.lse[orow] = lse2 * 0.69314718055994531f;
+        }
+#pragma unroll 1
+        for (int h = 0; h < HD / 32; ++h) {
+          uint32_t r[32];
+          __syncwarp();
+          tmem_ld32_wait(tO + h * 32, r);
+          float o[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = __uint_as_float(r[c]) * inv;
+          if (bad && live) {
+            // infinities and NaN that guard_v cleared, for the rows that see them
+            const int hidden = p.mask != nullptr ? g.ctx : g.ctx + g.i0 + 1;
+            for (int key = max(hidden, g.t0 * kBN); key < min(g.t1 * kBN, g.keys); ++key) {
+              const int j = key - g.ctx;
+              const bool seen = words != nullptr ? (j >> 5) < p.mask_words && (words[j >> 5] >> (j & 31) & 1u)
+                                                 : key < plain;
+              if (!seen) continue;
+              const int blk = p.table[g.request * p.table_stride + (key >> p.page_shift)];
+              if (blk < 0 || blk >= p.num_blocks) continue;
+              const T* vr = static_cast<const T*>(p.v) + blk * p.v_stride[0] +
+                            (key & ((1 << p.page_shift) - 1)) * p.v_stride[1] + g.head * p.v_stride[2] + 32 * h;
+#pragma unroll
+              for (int c = 0; c < 32; ++c) {
+                const float x = static_cast<float>(vr[c]);
+                if (!(fabsf(x) < INFINITY)) o[c] += x;
+              }
+            }
+          }
+          if (live) {
+            if (prow != nullptr) {
+#pragma unroll
+              for (int c = 0; c < 32; c += 4)
+                *reinterpret_cast<float4*>(prow + 32 * h + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+            } else {
+              uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + orow * HD + 32 * h);
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                to[c] = make_uint4(pack2<T>(o[8 * c], o[8 * c + 1]), pack2<T>(o[8 * c + 2], o[8 * c + 3]),
+                                   pack2<T>(o[8 * c + 4], o[8 * c + 5]), pack2<T>(o[8 * c + 6], o[8 * c + 7]));
+            }
+          }
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_ofree);
+      ++seg;
+    }
+
+    // rows of q that belong to no request (a batch padded to a fixed size)
+    const int end = p.requests > 0 ? max(0, min(p.cu[p.requests], p.tokens)) : 0;
+    const long long rows = static_cast<long long>(p.tokens - end) * p.heads;
+    for (long long r = static_cast<long long>(cta) * 4 + (warp - 4); r < rows; r += static_cast<long long>(p.grid) * 4) {
+      const long long orow = static_cast<long long>(end) * p.heads + r;
+      if (lane < HD / 8) reinterpret_cast<uint4*>(static_cast<T*>(p.out) + orow * HD)[lane] = make_uint4(0u, 0u, 0u, 0u);
+      if (p.lse != nullptr && lane == 0) p.lse[orow] = -INFINITY;
+    }
+  }
+
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the parts of the units that the division among CTAs cut: part k of
+// the unit that starts in CTA c is slot 2c + 1 (k = 0) or 2(c + k), and
+//   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M),  M = max_k lse_k.
+// A warp per row, lanes across the columns (D = 64: two parts at a time).
+constexpr int kJoinThreads = 256;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x;
+  const int4 cut = p.cuts[c];
+  const int parts = cut.x + 1;
+  if (parts <= 1) return;
   const int lane = threadIdx.x & 31;
-  const long long w = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  if (w >= a.tokens * a.heads) return;
-  const int t = static_cast<int>(w / a.heads), h = static_cast<int>(w % a.heads);
-  const int kh = h / static_cast<int>(a.heads / a.kv_heads);
-  int lo = 0, hi = static_cast<int>(a.requests);
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_seqlens[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  const int begin = a.cu_seqlens[lo], end = min(static_cast<long long>(a.cu_seqlens[lo + 1]), static_cast<long long>(a.tokens));
-  const int i = t - begin, count = end - begin;
-  constexpr int kPer = D / 32;
-  float q[kPer], o[kPer];
-  for (int e = 0; e < kPer; ++e) {
-    q[e] = static_cast<float>(static_cast<const T*>(a.q)[t * a.q_stride[0] + h * a.q_stride[1] + lane + 32 * e]);
-    o[e] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  if (begin >= 0 && i >= 0 && i < count) {
-    const int ctx = a.context_lens[lo];
-    long long keys = static_cast<long long>(ctx) + (a.tree_mask ? count : i + 1);
-    const long long room = a.table_cols << p.page_shift;
-    if (ctx < 0 || keys > room) {
-      if (lane == 0) atomicOr(p.err, kDevErrIndex);
-      keys = ctx < 0 ? 0 : room;
-    }
-    for (int j = 0; j < keys; ++j) {
-      if (j >= ctx && a.tree_mask) {
-        const int d = j - ctx;
-        if (d >= 32 * a.mask_words || !((a.tree_mask[t * a.mask_words + (d >> 5)] >> (d & 31)) & 1)) continue;
+  constexpr int kVecs = HD / 4, kAtOnce = 32 / kVecs;  // float4s per row, parts per pass
+  const int col = lane % kVecs, sub = lane / kVecs;
+  for (int row = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); row < cut.w; row += gridDim.y * (kJoinThreads / 32)) {
+    auto slot = [&](int k) { return k == 0 ? 2 * c + 1 : 2 * (c + k); };
+    float m = -INFINITY;
+    for (int k = lane; k < parts; k += 32) m = fmaxf(m, p.part_lse[slot(k) * kBM + row]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float m_use = m == -INFINITY ? 0.0f : m;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.0f;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      const float w = k0 + lane < parts ? ex2_approx(p.part_lse[slot(k0 + lane) * kBM + row] - m_use) : 0.0f;
+      sum += w;
+      const int here = min(32, parts - k0);
+#pragma unroll 8
+      for (int k = 0; k < here; k += kAtOnce) {
+        const float wk = __shfl_sync(0xffffffffu, w, (k + sub) & 31);
+        if (k + sub < here) {
+          const float4 v = reinterpret_cast<const float4*>(p.part + (static_cast<long long>(slot(k0 + k + sub)) * kBM + row) * HD)[col];
+          acc.x = fmaf(wk, v.x, acc.x);
+          acc.y = fmaf(wk, v.y, acc.y);
+          acc.z = fmaf(wk, v.z, acc.z);
+          acc.w = fmaf(wk, v.w, acc.w);
+        }
       }
-      const int block = a.block_table[lo * a.table_stride + (j >> p.page_shift)];
-      if (block < 0 || block >= a.num_blocks) {
-        if (lane == 0) atomicOr(p.err, kDevErrIndex);
-        continue;
-      }
-      const int r = j & ((1 << p.page_shift) - 1);
-      const T* kr = static_cast<const T*>(a.k_cache) + block * a.k_stride[0] + r * a.k_stride[1] + kh * a.k_stride[2];
-      const T* vr = static_cast<const T*>(a.v_cache) + block * a.v_stride[0] + r * a.v_stride[1] + kh * a.v_stride[2];
-      float s = 0.0f;
-      for (int e = 0; e < kPer; ++e) s = fmaf(q[e], static_cast<float>(kr[lane + 32 * e]), s);
-      for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= p.scale_log2;
-      const float mn = fmaxf(m, s);
-      const float alpha = (m == -INFINITY) ? 0.0f : ex2_approx(m - mn);
-      const float w_ = (mn == -INFINITY) ? 0.0f : ex2_approx(s - mn);
-      m = mn;
-      l = l * alpha + w_;
-      for (int e = 0; e < kPer; ++e) o[e] = o[e] * alpha + w_ * static_cast<float>(vr[lane + 32 * e]);
     }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+#pragma unroll
+    for (int d = 16; d >= kVecs; d >>= 1) {
+      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, d);
+      acc.y += __shfl_xor_sync(0xffffffffu, acc.y, d);
+      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, d);
+      acc.w += __shfl_xor_sync(0xffffffffu, acc.w, d);
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+    const long long orow = static_cast<long long>(cut.y + row / p.group) * p.heads + cut.z * p.group + row % p.group;
+    if (sub == 0)
+      reinterpret_cast<uint2*>(static_cast<T*>(p.out) + orow * HD)[col] =
+          make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    if (p.lse != nullptr && lane == 0)
+      p.lse[orow] = sum == 0.0f ? -INFINITY : (m_use + log2f(sum)) * 0.69314718055994531f;
   }
-  const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
-  for (int e = 0; e < kPer; ++e)
-    static_cast<T*>(a.out)[(static_cast<long long>(t) * a.heads + h) * D + lane + 32 * e] = static_cast<T>(o[e] * inv);
-  if (a.lse && lane == 0) a.lse[static_cast<long long>(t) * a.heads + h] = l != 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+size_t workspace_bytes(int grid, int64_t head_dim) {
+  const size_t slots = 2 * static_cast<size_t>(grid);
+  return slots * kBM * (head_dim + 1) * sizeof(float) + grid * sizeof(int4);
+}
+
+bool encode(CUtensorMap* tm, bool bf16, const void* base, int rank, const cuuint64_t* dims, const int64_t* strides,
+            const cuuint32_t* box) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return false;
+  cuuint64_t bytes[3];
+  cuuint32_t one[4] = {1, 1, 1, 1};
+  // the stride of a dimension of size 1 is never used, and torch gives it any value
+  for (int i = 0; i + 1 < rank; ++i) bytes[i] = dims[i + 1] == 1 ? dims[0] * 2 : static_cast<cuuint64_t>(strides[i]) * 2;
+  return enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base),
+             dims, bytes, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HD>
+cudaError_t launch(TreeParams& p, const fl_tree_attention_args& a, cudaStream_t stream) {
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kBN = Shape<HD>::kBN;
+  p.box_rows = static_cast<int>(std::min<int64_t>(a.page_size, kBN));
+  const cuuint64_t dq[3] = {HD, static_cast<cuuint64_t>(a.heads), static_cast<cuuint64_t>(a.tokens)};
+  const cuuint64_t dc[4] = {HD, static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(a.kv_heads),
+                            static_cast<cuuint64_t>(a.num_blocks)};
+  const int64_t sq[2] = {a.q_stride[1], a.q_stride[0]};
+  const int64_t sk[3] = {a.k_stride[1], a.k_stride[2], a.k_stride[0]}, sv[3] = {a.v_stride[1], a.v_stride[2], a.v_stride[0]};
+  const cuuint32_t bq[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(p.tile_tokens)};
+  const cuuint32_t bc[4] = {64, static_cast<cuuint32_t>(p.box_rows), 1, 1};
+  if (!encode(&p.tm_q, bf16, a.q, 3, dq, sq, bq) || !encode(&p.tm_k, bf16, a.k_cache, 4, dc, sk, bc) ||
+      !encode(&p.tm_v, bf16, a.v_cache, 4, dc, sv, bc))
+    return cudaErrorInvalidValue;
+  auto kern = tree_attention_kernel<T, HD>;
+  static std::atomic<bool> configured[kMaxFlagDevices];
+  cudaError_t e = ensure_smem_limit(kern, Shape<HD>::kSmemBytes, configured);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(kern, p.grid, kThreads, Shape<HD>::kSmemBytes, stream, p);
+  if (e != cudaSuccess) return e;
+  const int64_t rows = std::min<int64_t>(kBM, a.tokens * p.group);
+  const int ys = static_cast<int>(std::min<int64_t>(4, (rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32)));
+  return launch_pdl(tree_join_kernel<T, HD>, dim3(p.grid, ys), kJoinThreads, 0, stream, p);
 }
 
 int tree_attention(const fl_tree_attention_args* args, void* stream) {
@@ -103,45 +930,74 @@ int tree_attention(const fl_tree_attention_args* args, void* stream) {
     return fail(FL_ERR_UNSUPPORTED, "tree_attention requires head_dim 64 or 128");
   if (a.dtype != FL_DTYPE_F16 && a.dtype != FL_DTYPE_BF16)
     return fail(FL_ERR_UNSUPPORTED, "tree_attention supports fp16 and bf16");
-  if (a.kv_heads == 0 ? a.heads != 0 : (a.heads % a.kv_heads != 0 || a.heads / a.kv_heads > 128))
+  if (a.kv_heads == 0 ? a.heads != 0 : (a.heads % a.kv_heads != 0 || a.heads / a.kv_heads > kBM))
     return fail(FL_ERR_INVALID_ARGUMENT, "heads must be a multiple of kv_heads, at most 128 times");
   if (a.page_size < 8 || a.page_size > 256 || (a.page_size & (a.page_size - 1)) != 0)
     return fail(FL_ERR_UNSUPPORTED, "page_size must be a power of two from 8 to 256");
   if (a.requests > kMaxRequests) return fail(FL_ERR_UNSUPPORTED, "at most 4096 requests");
-  if (a.tokens > (1LL << 28) || a.heads > (1LL << 15) || a.num_blocks > 0x7fffffffLL || a.table_cols > (1LL << 26) ||
+  if (a.tokens > (1LL << 28) || a.heads > (1LL << 15) || a.num_blocks >= 0x7fffffffLL || a.table_cols > (1LL << 26) ||
       a.mask_words > (1LL << 20))
     return fail(FL_ERR_INVALID_ARGUMENT, "dimension too large");
   if (a.tokens == 0 || a.heads == 0) return FL_OK;
   if (!a.q || !a.out || !a.cu_seqlens || (a.requests > 0 && !a.context_lens) ||
       (a.requests > 0 && a.table_cols > 0 && !a.block_table) || (a.num_blocks > 0 && (!a.k_cache || !a.v_cache)))
     return fail(FL_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (a.num_blocks == 0) return fail(FL_ERR_INVALID_ARGUMENT, "empty cache");
+  if (!aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.out) || !aligned16(a.workspace))
+    return fail(FL_ERR_MISALIGNED, "q, the caches, out and workspace must be 16-byte aligned");
+  const int64_t sizes[8] = {a.tokens, a.heads, a.num_blocks, a.page_size, a.kv_heads, a.num_blocks, a.page_size, a.kv_heads};
+  const int64_t strides[8] = {a.q_stride[0], a.q_stride[1], a.k_stride[0], a.k_stride[1], a.k_stride[2],
+                              a.v_stride[0], a.v_stride[1], a.v_stride[2]};
+  for (int i = 0; i < 8; ++i)
+    if (sizes[i] > 1 && (strides[i] <= 0 || strides[i] % 8 != 0 || strides[i] >= (1LL << 39)))
+      return fail(FL_ERR_MISALIGNED, "strides of q and the caches must be positive multiples of 8 elements");
   int st = check_device();
   if (st != FL_OK) return st;
-  TreeParams p;
-  p.a = a;
+  TreeParams p = {};
+  p.grid = kCtasPerSm * sm_count();
+  if (!a.workspace || a.workspace_bytes < workspace_bytes(p.grid, a.head_dim))
+    return fail(FL_ERR_INVALID_ARGUMENT, "workspace too small (fl_tree_attention_workspace_size)");
+  p.v = a.v_cache;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.table = a.block_table;
+  p.context = a.context_lens;
+  p.cu = a.cu_seqlens;
+  p.mask = a.tree_mask != nullptr && a.mask_words > 0 ? a.tree_mask : nullptr;
+  p.part = static_cast<float*>(a.workspace);
+  p.part_lse = p.part + 2LL * p.grid * kBM * a.head_dim;
+  p.cuts = reinterpret_cast<int4*>(p.part_lse + 2LL * p.grid * kBM);
   p.err = device_error_word();
+  for (int i = 0; i < 3; ++i) p.v_stride[i] = a.v_stride[i];
+  p.table_stride = a.table_stride;
+  p.requests = static_cast<int>(a.requests);
+  p.tokens = static_cast<int>(a.tokens);
+  p.heads = static_cast<int>(a.heads);
+  p.kv_heads = static_cast<int>(a.kv_heads);
+  p.group = p.heads / p.kv_heads;
+  p.tile_tokens = kBM / p.group;
+  while ((1LL << p.page_shift) < a.page_size) ++p.page_shift;
+  p.num_blocks = static_cast<int>(a.num_blocks);
+  p.table_cols = static_cast<int>(a.table_cols);
+  p.mask_words = static_cast<int>(a.mask_words);
   double scale = a.sm_scale;
   if (scale == 0.0) scale = 1.0 / std::sqrt(static_cast<double>(a.head_dim));
   p.scale_log2 = static_cast<float>(scale * 1.44269504088896340736);
-  p.page_shift = 0;
-  while ((1LL << p.page_shift) < a.page_size) ++p.page_shift;
-  const long long warps = a.tokens * a.heads;
-  const int blocks = static_cast<int>((warps + kThreads / 32 - 1) / (kThreads / 32));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e;
-  if (a.dtype == FL_DTYPE_F16)
-    e = a.head_dim == 64 ? launch_pdl(tree_attention_kernel<__half, 64>, blocks, kThreads, 0, s, p)
-                         : launch_pdl(tree_attention_kernel<__half, 128>, blocks, kThreads, 0, s, p);
-  else
-    e = a.head_dim == 64 ? launch_pdl(tree_attention_kernel<__nv_bfloat16, 64>, blocks, kThreads, 0, s, p)
-                         : launch_pdl(tree_attention_kernel<__nv_bfloat16, 128>, blocks, kThreads, 0, s, p);
+  const cudaError_t e = a.dtype == FL_DTYPE_F16
+                            ? (a.head_dim == 64 ? launch<__half, 64>(p, a, s) : launch<__half, 128>(p, a, s))
+                            : (a.head_dim == 64 ? launch<__nv_bfloat16, 64>(p, a, s) : launch<__nv_bfloat16, 128>(p, a, s));
   return e == cudaSuccess ? FL_OK : cuda_fail(e, "tree attention launch");
 }
 
 }  // namespace
 }  // namespace fl
 
-extern "C" size_t fl_tree_attention_workspace_size(int64_t, int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t fl_tree_attention_workspace_size(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+  if (tokens <= 0 || heads <= 0 || kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  if (!fl::prepare_current_device()) return 0;
+  return fl::workspace_bytes(fl::kCtasPerSm * fl::sm_count(), head_dim);
+}
 
 extern "C" int fl_tree_attention(const fl_tree_attention_args* args, void* stream) {
   return fl::guarded([&] { return fl::tree_attention(args, stream); });
