@@ -9,12 +9,20 @@
 // The same kernel appends to a paged cache: rotated keys and unchanged values
 // go to the rows that the slot map names instead of to k_out.
 //
-// Bound by memory: each element is read and written once. A lane owns 2 * VEC
-// columns of a row (two 16-byte accesses) as A[VEC], B[VEC] of VEC pairs, and
-// keeps their cosines and sines in registers while it walks over the heads,
-// so the table is read once per token and warp, not once per head. The lanes
-// of a warp that the columns of one row leave over take further heads where
-// heads are closer together in memory than tokens, further tokens otherwise.
+// Bound by memory: each element is read and written once. A lane owns two
+// 16-byte vectors of a row and walks over a token's heads with their cosines
+// and sines in registers, so the table is read once per token and warp, not
+// once per head. The lanes of a warp that the columns of one row leave over
+// take further heads where heads are closer together in memory than tokens,
+// further tokens otherwise. What it takes is bytes under way: through
+// registers, two heads at a time at 24 warps per SM, a training step's q and
+// k of 1 GB ran at 5.1 TB/s; with asynchronous copies into slots of shared
+// memory that are each thread's own, four heads ahead, at 6.6 TB/s (153 us
+// for 3 x 16381 tokens of 32 + 8 heads of 128, bf16; a copy of as many bytes
+// 154 us), 8191 tokens of 32 + 8 + 8 heads appended to a cache 58 -> 36 us.
+// Interleaved pairs need whole vectors side by side across the lanes: with
+// both vectors of a lane side by side, each access used half of each sector
+// (223 us for the 153).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -23,187 +31,265 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "../../include/flashlite_b200.h"
 #include "fl_internal.h"
 #include "fl_ptx.cuh"
+#include "fl_types.cuh"
 
 namespace fl {
 namespace {
 
 constexpr int kThreads = 256;
 
+// Heads of a lane under way, and blocks per SM: 4 x 32 bytes x 768 threads =
+// 96 KB per SM. Depths of 3 and 8, and 4 blocks (fewer registers), measured
+// within 5 % of it over the sizes below.
+constexpr int kDepth = 4;
+constexpr int kBlocksPerSm = 3;
+constexpr int kWarpsPerSm = 16;  // what fills the GPU
+
 struct RotaryParams {
   fl_rotary_args a;
   unsigned int* err;
   int lanes;       // lanes per row: a power of two
-  int units;       // (2 * VEC)-column units per row
-  int rot_units;   // of which rotated
+  int units;       // units of two vectors per row
+  int rot_units;   // of which rotated (half layout)
   int over_heads;  // what a warp's further lane groups take: heads (1) or tokens (0)
-  int chunk;       // heads a warp walks over
-  int n_chunks;
   int heads;       // q, k and v heads together
-  long long warps; // warps with work
+  int chunk;       // of which a warp takes so many
+  uint32_t n_chunks, tokens, length, warps;  // chunks; warps with work
 };
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T x) { return static_cast<float>(x); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
+// Asynchronous 16-byte copy to shared memory, past L1.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Turns pairs. Half layout: x has the first column of VEC pairs and y the
+// second. Interleaved: x and y hold VEC / 2 pairs each, (0, 1), (2, 3), ...,
+// turned if tx, ty; the angles of y's pairs follow those of x's. (Single
+// elements, VEC = 1, are one pair either way.) 16-bit types go through
+// registers two elements at a time.
+template <typename T, int VEC, bool kInterleaved>
+__device__ __forceinline__ void turn(Pack<T, VEC>& x, Pack<T, VEC>& y, const float (&c)[VEC], const float (&s)[VEC],
+                                     bool tx, bool ty) {
+  if constexpr (VEC == 8) {
+    uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
+    uint32_t* yw = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 e = unpack2<T>(xw[j]), f = unpack2<T>(yw[j]);
+      if constexpr (kInterleaved) {
+        if (tx) xw[j] = pack2<T>(fmaf(e.x, c[j], -(e.y * s[j])), fmaf(e.y, c[j], e.x * s[j]));
+        if (ty) yw[j] = pack2<T>(fmaf(f.x, c[j + 4], -(f.y * s[j + 4])), fmaf(f.y, c[j + 4], f.x * s[j + 4]));
+      } else if (tx) {
+        xw[j] = pack2<T>(fmaf(e.x, c[2 * j], -(f.x * s[2 * j])), fmaf(e.y, c[2 * j + 1], -(f.y * s[2 * j + 1])));
+        yw[j] = pack2<T>(fmaf(f.x, c[2 * j], e.x * s[2 * j]), fmaf(f.y, c[2 * j + 1], e.y * s[2 * j + 1]));
+      }
+    }
+  } else if constexpr (kInterleaved && VEC > 1) {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {
+      const float x0 = x.v[2 * j], x1 = x.v[2 * j + 1], y0 = y.v[2 * j], y1 = y.v[2 * j + 1];
+      if (tx) {
+        x.v[2 * j] = fmaf(x0, c[j], -(x1 * s[j]));
+        x.v[2 * j + 1] = fmaf(x1, c[j], x0 * s[j]);
+      }
+      if (ty) {
+        y.v[2 * j] = fmaf(y0, c[VEC / 2 + j], -(y1 * s[VEC / 2 + j]));
+        y.v[2 * j + 1] = fmaf(y1, c[VEC / 2 + j], y0 * s[VEC / 2 + j]);
+      }
+    }
+  } else if (tx) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float x0 = static_cast<float>(x.v[j]), x1 = static_cast<float>(y.v[j]);
+      x.v[j] = static_cast<T>(fmaf(x0, c[j], -(x1 * s[j])));
+      y.v[j] = static_cast<T>(fmaf(x1, c[j], x0 * s[j]));
+    }
+  }
+}
+
 // One row's address: token (b, n) and head h of a tensor [B, N, H, D] given
 // by its strides in elements.
-template <typename T>
 __device__ __forceinline__ long long row_of(const int64_t (&st)[3], long long b, long long n, int h) {
   return b * st[0] + n * st[1] + static_cast<long long>(h) * st[2];
 }
 
 template <typename T, int VEC, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_kernel(const __grid_constant__ RotaryParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long w = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t w = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (w >= p.warps) return;
   const fl_rotary_args& a = p.a;
   const int lane = threadIdx.x & 31;
   const int groups = 32 / p.lanes;
-  const int g = lane / p.lanes;
-  const int u0 = lane % p.lanes;
-  const long long tokens = a.batch * a.length;
-  const long long tw = w / p.n_chunks;
-  const int h0 = static_cast<int>(w % p.n_chunks) * p.chunk;
-  const int h1 = min(h0 + p.chunk, p.heads);
-  const long long t = p.over_heads ? tw : tw * groups + g;
-  if (t >= tokens) return;
+  const int g = lane / p.lanes, u0 = lane % p.lanes;
+  const uint32_t tw = w / p.n_chunks, chunk = w - tw * p.n_chunks;
+  const uint32_t t = p.over_heads ? tw : tw * groups + g;
+  if (t >= p.tokens) return;
+  const uint32_t b = t / p.length, n = t - b * p.length;
   const int hstep = p.over_heads ? groups : 1;
-  const long long b = t / a.length, n = t % a.length;
+  const int hq = static_cast<int>(a.heads), hk = static_cast<int>(a.kv_heads);
+  const int h0 = chunk * p.chunk;
 
-  const long long pi = (a.positions_batch ? t : n);
+  const uint32_t pi = a.positions_batch ? t : n;
   const long long pos = a.positions == nullptr ? n
                         : a.positions_64 ? static_cast<const int64_t*>(a.positions)[pi]
                                          : static_cast<const int32_t*>(a.positions)[pi];
   const bool known = pos >= 0 && pos < a.table_rows;
-  if (!known && u0 == 0 && p.err) atomicOr(p.err, kDevErrIndex);
+  if (!known && a.rot > 0 && u0 == 0 && p.err) atomicOr(p.err, kDevErrIndex);
   long long kc = 0, vc = 0;  // the token's row in the caches
   bool cached = false;
   if (a.slots != nullptr) {
     const long long slot = a.slots[t];
     cached = slot >= 0 && slot < a.cache_blocks * a.page_size;
-    if (!cached && slot != -1 && u0 == 0 && p.err) atomicOr(p.err, kDevErrIndex);
     if (cached) {
-      const long long blk = slot / a.page_size, r = slot % a.page_size;
+      const long long blk = ((slot | a.page_size) >> 32) == 0
+                                ? static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.page_size)
+                                : slot / a.page_size;
+      const long long r = slot - blk * a.page_size;
       kc = blk * a.k_out_stride[0] + r * a.k_out_stride[1];
       vc = blk * a.v_out_stride[0] + r * a.v_out_stride[1];
+    } else if (slot != -1 && u0 == 0 && p.err) {
+      atomicOr(p.err, kDevErrIndex);
     }
   }
-  const int hq = static_cast<int>(a.heads), hk = static_cast<int>(a.kv_heads);
+
+  const T* q_in = static_cast<const T*>(a.q) + row_of(a.q_stride, b, n, 0);
+  const T* k_in = static_cast<const T*>(a.k) + row_of(a.k_stride, b, n, 0);
+  const T* v_in = static_cast<const T*>(a.v) + row_of(a.v_stride, b, n, 0);
+  T* q_out = static_cast<T*>(a.q_out) + row_of(a.q_out_stride, b, n, 0);
+  T* k_out = static_cast<T*>(a.k_out) + (a.slots == nullptr ? row_of(a.k_out_stride, b, n, 0) : kc);
+  T* v_out = static_cast<T*>(a.v_out) + vc;
+  // a token without a slot has only its q heads
+  const int last = min(h0 + p.chunk, a.slots == nullptr || cached ? p.heads : hq);
 
   for (int u = u0; u < p.units; u += p.lanes) {
-    const bool turned = u < p.rot_units;
-    // columns of A and B; in the scalar form an odd D leaves a unit without B
-    const int ca = turned && !kInterleaved ? u * VEC : u * 2 * VEC;
-    const int cb = turned && !kInterleaved ? static_cast<int>(a.rot / 2) + u * VEC : ca + VEC;
-    const bool has_b = cb < a.head_dim;
-    float c[VEC], s[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      c[j] = 1.0f;
-      s[j] = 0.0f;
+    // The unit's two vectors A and B: neighbouring lanes take neighbouring
+    // vectors, so that each access of a warp covers whole sectors.
+    const int rot = static_cast<int>(a.rot), dim = static_cast<int>(a.head_dim);
+    int ca, cb;
+    if (VEC > 1 && kInterleaved) {
+      ca = u * VEC;
+      cb = dim / 2 + ca;
+    } else if (kInterleaved) {
+      ca = 2 * u;
+      cb = ca + 1;
+    } else if (u < p.rot_units) {
+      ca = u * VEC;
+      cb = rot / 2 + ca;
+    } else {  // columns that are copied
+      const int left = (dim - rot + 2 * VEC - 1) / (2 * VEC);
+      ca = rot + (u - p.rot_units) * VEC;
+      cb = ca + left * VEC;
     }
-    if (turned) {
-      if (known) {
-        const float* row = a.table + pos * a.rot;
-        if constexpr (VEC >= 4) {
+    const bool has_b = cb < dim;  // single elements: an odd number of copied columns leaves one without
+    const bool turn_a = ca < rot, turn_b = cb < rot;
+    float c[VEC], s[VEC];
+    auto angles = [&] {
 #pragma unroll
-          for (int j = 0; j < VEC; j += 4) {
-            const float4 cc = __ldg(reinterpret_cast<const float4*>(row + u * VEC + j));
-            const float4 ss = __ldg(reinterpret_cast<const float4*>(row + a.rot / 2 + u * VEC + j));
-            c[j] = cc.x; c[j + 1] = cc.y; c[j + 2] = cc.z; c[j + 3] = cc.w;
-            s[j] = ss.x; s[j + 1] = ss.y; s[j + 2] = ss.z; s[j + 3] = ss.w;
+      for (int j = 0; j < VEC; ++j) c[j] = s[j] = __int_as_float(0x7fc00000);
+      if (!known) return;  // a position outside the table leaves NaN: nothing to turn by, and not to be missed
+      const float* row = a.table + pos * a.rot;
+      auto get = [&](int pair, int j, auto count) {  // the angles of `count` pairs into c[j], s[j] on
+        constexpr int kCount = decltype(count)::value;
+        if constexpr (kCount % 4 == 0) {
+#pragma unroll
+          for (int e = 0; e < kCount; e += 4) {
+            const float4 cc = __ldg(reinterpret_cast<const float4*>(row + pair + e));
+            const float4 ss = __ldg(reinterpret_cast<const float4*>(row + rot / 2 + pair + e));
+            c[j + e] = cc.x; c[j + e + 1] = cc.y; c[j + e + 2] = cc.z; c[j + e + 3] = cc.w;
+            s[j + e] = ss.x; s[j + e + 1] = ss.y; s[j + e + 2] = ss.z; s[j + e + 3] = ss.w;
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            c[j] = row[u * VEC + j];
-            s[j] = row[a.rot / 2 + u * VEC + j];
+          for (int e = 0; e < kCount; ++e) {
+            c[j + e] = row[pair + e];
+            s[j + e] = row[rot / 2 + pair + e];
           }
         }
-        if (a.inverse) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) s[j] = -s[j];
-        }
-      } else {  // a position outside the table: nothing to turn by, and not to be missed
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) c[j] = s[j] = __int_as_float(0x7fc00000);
+      };
+      if constexpr (VEC > 1 && kInterleaved) {
+        if (turn_a) get(ca / 2, 0, std::integral_constant<int, VEC / 2>{});
+        if (turn_b) get(cb / 2, VEC / 2, std::integral_constant<int, VEC / 2>{});
+      } else if (turn_a) {
+        get(u * VEC, 0, std::integral_constant<int, VEC>{});
       }
-    }
-#pragma unroll 4
-    for (int h = h0 + (p.over_heads ? g : 0); h < h1; h += hstep) {
+      if (a.inverse) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s[j] = -s[j];
+      }
+    };
+    // The lane's heads one after the other: head `it` of q, then k, then v.
+    const int first = h0 + (p.over_heads ? g : 0);
+    struct Place {
       const T* src;
       T* dst;
-      bool rotate = turned;
-      if (h < hq) {
-        src = static_cast<const T*>(a.q) + row_of<T>(a.q_stride, b, n, h);
-        dst = static_cast<T*>(a.q_out) + row_of<T>(a.q_out_stride, b, n, h);
-      } else if (h < hq + hk) {
-        src = static_cast<const T*>(a.k) + row_of<T>(a.k_stride, b, n, h - hq);
-        if (a.slots != nullptr) {
-          if (!cached) continue;
-          dst = static_cast<T*>(a.k_out) + kc + (h - hq) * a.k_out_stride[2];
-        } else {
-          dst = static_cast<T*>(a.k_out) + row_of<T>(a.k_out_stride, b, n, h - hq);
+      bool rotated;  // not v
+    };
+    auto place = [&](int h) -> Place {
+      if (h < hq) return {q_in + h * a.q_stride[2], q_out + h * a.q_out_stride[2], true};
+      h -= hq;
+      if (h < hk) return {k_in + h * a.k_stride[2], k_out + h * a.k_out_stride[2], true};
+      h -= hk;
+      return {v_in + h * a.v_stride[2], v_out + h * a.v_out_stride[2], false};
+    };
+    if constexpr (VEC * sizeof(T) == 16) {
+      // kDepth heads are under way in slots of shared memory that are this
+      // thread's own, so no barrier is needed. (Outputs may be the inputs:
+      // no element is anyone else's.)
+      extern __shared__ __align__(16) uint4 slots[];
+      const uint32_t mine = smem_u32(slots + threadIdx.x);
+      auto fetch = [&](int h, int i) {
+        if (h < last) {
+          const T* src = place(h).src;
+          copy16(mine + (2 * i) * (kThreads * 16), src + ca);
+          copy16(mine + (2 * i + 1) * (kThreads * 16), src + cb);
         }
-      } else {
-        if (!cached) continue;
-        src = static_cast<const T*>(a.v) + row_of<T>(a.v_stride, b, n, h - hq - hk);
-        dst = static_cast<T*>(a.v_out) + vc + (h - hq - hk) * a.v_out_stride[2];
-        rotate = false;
+        copy_commit();
+      };
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) fetch(first + i * hstep, i);
+      angles();
+      int i = 0;
+#pragma unroll 1
+      for (int h = first; h < last; h += hstep) {
+        copy_wait<kDepth - 1>();
+        Pack<T, VEC> x, y;
+        *reinterpret_cast<uint4*>(&x) = slots[(2 * i) * kThreads + threadIdx.x];
+        *reinterpret_cast<uint4*>(&y) = slots[(2 * i + 1) * kThreads + threadIdx.x];
+        const Place at = place(h);
+        if (at.rotated) turn<T, VEC, kInterleaved>(x, y, c, s, turn_a, turn_b);
+        *reinterpret_cast<uint4*>(at.dst + ca) = *reinterpret_cast<const uint4*>(&x);
+        *reinterpret_cast<uint4*>(at.dst + cb) = *reinterpret_cast<const uint4*>(&y);
+        fetch(h + kDepth * hstep, i);
+        i = i + 1 == kDepth ? 0 : i + 1;
       }
-      Pack<T, VEC> x, y;
-      x = *reinterpret_cast<const Pack<T, VEC>*>(src + ca);
-      y = x;
-      if (has_b) y = *reinterpret_cast<const Pack<T, VEC>*>(src + cb);
-      if (rotate) {
-        if constexpr (kInterleaved) {  // x, y hold 2 * VEC neighbouring columns: pairs (0,1), (2,3), ...
-          T e[2 * VEC];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            e[j] = x.v[j];
-            e[VEC + j] = y.v[j];
-          }
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float x0 = to_f32(e[2 * j]), x1 = to_f32(e[2 * j + 1]);
-            e[2 * j] = from_f32<T>(fmaf(x0, c[j], -(x1 * s[j])));
-            e[2 * j + 1] = from_f32<T>(fmaf(x1, c[j], x0 * s[j]));
-          }
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            x.v[j] = e[j];
-            y.v[j] = e[VEC + j];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float x0 = to_f32(x.v[j]), x1 = to_f32(y.v[j]);
-            x.v[j] = from_f32<T>(fmaf(x0, c[j], -(x1 * s[j])));
-            y.v[j] = from_f32<T>(fmaf(x1, c[j], x0 * s[j]));
-          }
-        }
+      copy_wait<0>();
+    } else {
+      angles();
+      for (int h = first; h < last; h += hstep) {
+        const Place at = place(h);
+        Pack<T, VEC> x, y;
+        x.v[0] = at.src[ca];
+        y.v[0] = x.v[0];
+        if (has_b) y.v[0] = at.src[cb];
+        if (at.rotated) turn<T, VEC, kInterleaved>(x, y, c, s, turn_a, turn_b);
+        at.dst[ca] = x.v[0];
+        if (has_b) at.dst[cb] = y.v[0];
       }
-      *reinterpret_cast<Pack<T, VEC>*>(dst + ca) = x;
-      if (has_b) *reinterpret_cast<Pack<T, VEC>*>(dst + cb) = y;
     }
   }
 }
@@ -227,19 +313,25 @@ cudaError_t launch(const fl_rotary_args& a, cudaStream_t stream) {
   p.over_heads = near[2] <= near[1] ? 1 : 0;
   const long long tokens = a.batch * a.length;
   const long long rows = p.over_heads ? tokens : (tokens + groups - 1) / groups;
-  // A warp walks over all heads of its tokens where that leaves enough warps
-  // to fill the GPU (16 per SM); with fewer tokens the heads are divided too.
+  // A warp takes all heads of its tokens where that leaves enough warps to
+  // fill the GPU; with fewer tokens the heads are divided too.
   const int hstep = p.over_heads ? groups : 1;
   const int steps = (p.heads + hstep - 1) / hstep;
-  const long long want = 16LL * sm_count();
+  const long long want = static_cast<long long>(kWarpsPerSm) * sm_count();
   const long long split = std::min<long long>(steps, std::max<long long>(1, (want + rows - 1) / rows));
   p.chunk = static_cast<int>((steps + split - 1) / split) * hstep;
-  p.n_chunks = (p.heads + p.chunk - 1) / p.chunk;
-  p.warps = rows * p.n_chunks;
-  const long long blocks = (p.warps + kThreads / 32 - 1) / (kThreads / 32);
-  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  return a.interleaved ? launch_pdl(rotary_kernel<T, VEC, true>, static_cast<int>(blocks), kThreads, 0, stream, p)
-                       : launch_pdl(rotary_kernel<T, VEC, false>, static_cast<int>(blocks), kThreads, 0, stream, p);
+  p.n_chunks = static_cast<uint32_t>((p.heads + p.chunk - 1) / p.chunk);
+  const long long warps = rows * p.n_chunks;
+  if (warps > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  p.tokens = static_cast<uint32_t>(tokens);
+  p.length = static_cast<uint32_t>(a.length);
+  p.warps = static_cast<uint32_t>(warps);
+  const int blocks = static_cast<int>((warps + kThreads / 32 - 1) / (kThreads / 32));
+  auto kern = a.interleaved ? rotary_kernel<T, VEC, true> : rotary_kernel<T, VEC, false>;
+  constexpr int smem = VEC > 1 ? 2 * kDepth * kThreads * 16 : 0;
+  static std::atomic<bool> configured[2][kMaxFlagDevices];
+  const cudaError_t e = ensure_smem_limit(kern, smem, configured[a.interleaved ? 1 : 0]);
+  return e == cudaSuccess ? launch_pdl(kern, blocks, kThreads, smem, stream, p) : e;
 }
 
 template <typename T>
