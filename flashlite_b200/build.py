@@ -26,7 +26,8 @@ BUILD = PKG / "_build"
 CUDA_SOURCES = ["fl_api.cu", "fl_flash2.cu", "fl_flash2_sk.cu", "fl_flash2_bwd.cu", "fl_naive.cu",
                 "fl_noalloc.cu", "fl_selftest.cu", "fl_rotary.cu", "fl_plan.cu", "fl_tree.cu"]
 BINDING_SOURCES = ["flash_attn.cpp", "serving.cpp"]
-HEADERS = ["fl_ptx.cuh", "fl_internal.h", "fl_flash2_common.cuh", "fl_types.cuh"]
+HEADERS = ["fl_ptx.cuh", "fl_internal.h", "fl_flash2_common.cuh", "fl_tree_common.cuh",
+           "fl_types.cuh"]
 LIB = PKG / "libflashlite_b200.so"
 EXT = PKG / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 

@@ -6,17 +6,10 @@
 //   the new ones that its mask (or the causal rule) names. m_t is a running
 //   reference maximum; a row that sees nothing gives 0 and -inf.
 //
-// A unit of work is (request, key head, row tile): up to 128 rows, the
-// request's tokens times the query heads that share the key head, so that
-// each key and value is read once for all of them. Rows that a short request
-// leaves empty cost nothing in the memory-bound case: the tensor cores finish
-// a 128-row product in a fraction of the time its keys take to arrive, and
-// softmax warps without rows skip it. A unit's keys are cut into tiles (kBN
-// keys, gathered page by page with TMA); all tiles of all units, laid end to
-// end, are divided evenly among the CTAs whatever the requests' lengths, which
-// the kernel reads on the device. A CTA that ends up with part of a unit
-// leaves an fp32 partial result, and a second kernel joins the parts of each
-// cut unit in order (no atomics: the same bits every time).
+// fl_tree_common.cuh has the units of work and their division. This file has
+// the entry point and the kernel: units of up to 128 rows, S = Q K^T and
+// O += P V as 128-row products, keys and values gathered page by page with
+// TMA.
 //
 // A CTA is a scheduler warp, K and V producer warps, an MMA warp and one
 // softmax warpgroup, one thread per row; two CTAs share an SM and fill each
@@ -29,19 +22,11 @@
 // infinities and NaN, which are cleared too and added back, in the epilogue,
 // to the rows that see them.
 
-#include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
 #include <algorithm>
 #include <cmath>
-#include <cstdint>
 #include <string>
 
-#include "../../include/flashlite_b200.h"
-#include "fl_internal.h"
-#include "fl_ptx.cuh"
+#include "fl_tree_common.cuh"
 
 namespace fl {
 namespace {
@@ -50,13 +35,8 @@ constexpr int kThreads = 256;
 constexpr int kBM = 128;           // rows per unit (UMMA M)
 constexpr int kMaxRequests = 4096;
 constexpr uint32_t kTmemCols = 256;
-constexpr int kSegRing = 4;        // work descriptors between the scheduler and the other warps
 constexpr int kSegReaders = 7;     // K, V, MMA and four softmax warps
 constexpr int kCtasPerSm = 2;
-// Fewest tiles worth a CTA of their own.
-#ifndef FL_TREE_MIN_STEPS
-#define FL_TREE_MIN_STEPS 1
-#endif
 
 // Shape per head dimension; tiles are made of 64-column (128-byte) swizzle
 // atoms as in the other forward kernels. K and V tiles are 16 KB both ways;
@@ -83,150 +63,86 @@ struct Shape {
 // Register split: 128 x 64 (producers, MMA, scheduler) + 128 x 192 (softmax) = 256 x 128, the launch's total.
 constexpr int kRegsProducer = 64, kRegsSoftmax = 192;
 
-// A reference maximum is kept until a row's maximum exceeds it by this much
-// (log2); probabilities are held 2^kUp times their size, so that fp16 keeps
-// the small ones out of its subnormal range: at most 2^15 after the lag.
-constexpr float kLag = 8.0f, kUp = 7.0f;
-
-struct TreeParams {
-  CUtensorMap tm_q;  // {D, heads, tokens}, box {64, group, tokens per row tile}
-  CUtensorMap tm_k;  // {D, page rows, key heads, blocks}, box {64, min(page, kBN), 1, 1}
-  CUtensorMap tm_v;
-  const void* v;
-  void* out;
-  float* lse;
-  const int32_t* table;
-  const int32_t* context;
-  const int32_t* cu;
-  const uint32_t* mask;
-  float* part;       // [2 * grid][128][D] fp32, then [2 * grid][128] log2-sum-exp
-  float* part_lse;
-  int4* cuts;        // [grid]: parts after the first, first token, head and rows of the cut unit that starts there
-  unsigned int* err;
-  long long v_stride[3];
-  long long table_stride;
-  int requests, tokens, heads, kv_heads, group, tile_tokens;
-  int page_shift, box_rows, num_blocks, table_cols, mask_words;
-  float scale_log2;
-  int grid;
-};
-
-// One request as the schedule sees it.
-struct Request {
-  int begin, count, ctx, room;  // first row of q, new tokens, cached tokens, keys its table row can name
-};
-
-__device__ __forceinline__ Request request_of(const TreeParams& p, int begin, int end, int ctx, bool report) {
-  Request r;
-  const long long room = static_cast<long long>(p.table_cols) << p.page_shift;
-  r.room = room > 0x3fffffff ? 0x3fffffff : static_cast<int>(room);
-  bool sound = true;
-  r.begin = begin;
-  r.count = end - begin;
-  if (begin < 0 || end < begin || end > p.tokens) {
-    sound = false;
-    r.begin = r.count = 0;
-  }
-  r.ctx = ctx;
-  if (ctx < 0 || ctx > r.room) {
-    sound = false;
-    r.ctx = ctx < 0 ? 0 : r.room;
-  }
-  if (r.count > r.room - r.ctx) sound = false;  // the new tokens past the table's end are not visible
-  if (!sound && report) atomicOr(p.err, kDevErrIndex);
-  return r;
-}
-
-// Keys that some row of the row tile with tokens [i0, i0 + n) may see.
-__device__ __forceinline__ int keys_of(const TreeParams& p, const Request& r, int i0) {
-  int inner;
-  if (p.mask != nullptr) inner = min(r.count, 32 * p.mask_words);
-  else inner = min(r.count, i0 + p.tile_tokens);
-  return min(r.ctx + inner, r.room);
-}
-
-template <int kBN>
-__device__ __forceinline__ int tiles_of(const TreeParams& p, const Request& r, int i0) {
-  return max(1, (keys_of(p, r, i0) + kBN - 1) / kBN);
-}
-
-// Tiles of one key head of a request: those of all its row tiles.
-template <int kBN>
-__device__ __forceinline__ long long head_tiles(const TreeParams& p, const Request& r) {
-  if (r.count == 0) return 0;
-  if (p.mask != nullptr)
-    return static_cast<long long>((r.count + p.tile_tokens - 1) / p.tile_tokens) * tiles_of<kBN>(p, r, 0);
-  long long n = 0;
-  for (int i0 = 0; i0 < r.count; i0 += p.tile_tokens) n += tiles_of<kBN>(p, r, i0);
-  return n;
-}
-
-// A CTA's share of one unit: tiles [t0, t1) of n.
-struct Segment {
-  int request, head, i0, rows;  // rows = tokens in the row tile times group
-  int begin, count, ctx, keys;
-  int t0, t1;                   // t1 < 0: no more work
-  int slot;                     // partial result, -1: the whole unit, written to out
-  int pad;
-};
-
-__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err));
-}
-__device__ __forceinline__ bool wait_all_issuer(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                                unsigned int* err) {
-  return __all_sync(0xffffffffu, mbar_wait_issuer(bar, parity, abort_flag, err));
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
-
-// Exponent bits of the type, all set in infinities and NaN.
-template <typename T>
-constexpr uint32_t kExpBits = 0x7C00u;
-template <>
-constexpr uint32_t kExpBits<__nv_bfloat16> = 0x7F80u;
-
-// A pair with its infinite and NaN elements cleared.
-template <typename T>
-__device__ __forceinline__ uint32_t finite2(uint32_t w) {
-  constexpr uint32_t e = kExpBits<T>;
-  if ((w & e) == e) w &= 0xffff0000u;
-  if ((w >> 16 & e) == e) w &= 0x0000ffffu;
-  return w;
-}
-
-__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-
-// Makes a V tile safe for the product, by one warp: rows [valid, kBN) cleared,
-// infinities and NaN in rows [mixed, valid) cleared. Returns whether any were.
+// Joins the n partial results base, base + stride, ... of a unit:
+//   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M),  M = max_k lse_k,
+// by the 128 softmax threads; into slot `to` or, if to < 0, out. Part i of a
+// unit that begins in CTA `first` is slot 2 first + 1 (i = 0) or 2 (first + i).
+// Neighbouring threads take neighbouring rows (the layout of a slot is
+// [D / 4][128] float4), and the columns that few rows leave threads for.
+// Returns the joined log2-sum-exp of row tid, if tid < rows.
 template <typename T, int HD>
-__device__ __forceinline__ bool guard_v(uint32_t tile, int mixed, int valid, int lane) {
-  constexpr int kBN = Shape<HD>::kBN;
-  bool bad = false;
+__device__ __forceinline__ float join_parts(const TreeParams& p, const Segment& g, int tid, int first, int base, int stride,
+                                            int n, int to) {
+  constexpr int kVecs = HD / 4;
+  int span = 1;  // rows, as a power of two
+  while (span < g.rows) span *= 2;
+  const int row = tid & (span - 1), lanes = kBM / span, c0 = tid / span;
+  if (row >= g.rows || c0 >= kVecs) return 0.0f;
+  const int token = g.begin + g.i0 + row / p.group, head = g.head * p.group + row % p.group;
+  const long long orow = static_cast<long long>(token) * p.heads + head;
+  float lse2 = 0.0f;
+  // kCols columns of kBatch parts at a time, all their loads under way
+  // together; M is a running maximum. Rolled otherwise: on its first run in a
+  // kernel, code costs as much to fetch as to execute.
+  auto join = [&](auto cols, auto batch) {
+    constexpr int kCols = decltype(cols)::value, kBatch = decltype(batch)::value;
+#pragma unroll 1
+    for (int c = c0; c < kVecs; c += kCols * lanes) {
+      float4 acc[kCols];
+      float m = -INFINITY, sum = 0.0f;
 #pragma unroll
-  for (int hh = 0; hh < Shape<HD>::kHalves; ++hh) {
-    const uint32_t half = tile + hh * (kBN * 128);
-    for (int c = valid * 8 + lane; c < kBN * 8; c += 32) st_shared_v4(half + c * 16, 0u, 0u, 0u, 0u);
-    for (int c = mixed * 8 + lane; c < valid * 8; c += 32) {
-      const uint4 v = ld_shared_v4(half + c * 16);
-      const uint4 f = make_uint4(finite2<T>(v.x), finite2<T>(v.y), finite2<T>(v.z), finite2<T>(v.w));
-      if (f.x != v.x || f.y != v.y || f.z != v.z || f.w != v.w) {
-        st_shared_v4(half + c * 16, f.x, f.y, f.z, f.w);
-        bad = true;
+      for (int j = 0; j < kCols; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int k0 = 0; k0 < n; k0 += kBatch) {
+        float l[kBatch];
+        float4 v[kBatch][kCols];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const bool in = k0 + k < n;
+          const int sl = slot_of(first, base + min(k0 + k, n - 1) * stride);
+          l[k] = in ? __ldcg(p.part_lse + sl * kBM + row) : -INFINITY;
+          const float4* from = reinterpret_cast<const float4*>(p.part) + static_cast<long long>(sl) * kVecs * kBM + row;
+#pragma unroll
+          for (int j = 0; j < kCols; ++j)
+            v[k][j] = in && c + j * lanes < kVecs ? __ldcg(from + (c + j * lanes) * kBM) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float m_new = m;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, l[k]);
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new, alpha = ex2_approx(m - m_use);
+        m = m_new;
+        sum *= alpha;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+          acc[j] = make_float4(acc[j].x * alpha, acc[j].y * alpha, acc[j].z * alpha, acc[j].w * alpha);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const float w = ex2_approx(l[k] - m_use);
+          sum += w;
+#pragma unroll
+          for (int j = 0; j < kCols; ++j)
+            acc[j] = make_float4(fmaf(w, v[k][j].x, acc[j].x), fmaf(w, v[k][j].y, acc[j].y), fmaf(w, v[k][j].z, acc[j].z),
+                                 fmaf(w, v[k][j].w, acc[j].w));
+        }
+      }
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        if (c + j * lanes >= kVecs) break;
+        const float4 o = make_float4(acc[j].x * inv, acc[j].y * inv, acc[j].z * inv, acc[j].w * inv);
+        if (to >= 0)
+          reinterpret_cast<float4*>(p.part)[(static_cast<long long>(to) * kVecs + c + j * lanes) * kBM + row] = o;
+        else
+          reinterpret_cast<uint2*>(static_cast<T*>(p.out) + orow * HD)[c + j * lanes] =
+              make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
       }
     }
-  }
-  fence_proxy_async_smem();
-  return __any_sync(0xffffffffu, bad);
+  };
+  if (lanes * 4 <= kVecs) join(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+  else join(std::integral_constant<int, 1>{}, std::integral_constant<int, 6>{});
+  if (c0 == 0 && to < 0 && p.lse != nullptr) p.lse[orow] = lse2 * 0.69314718055994531f;
+  return lse2;
 }
 
 template <typename T, int HD>
@@ -238,29 +154,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
   const uint32_t s_q = sbase + C::kSmemQ, s_k0 = sbase + C::kSmemK, s_v0 = sbase + C::kSmemV;
-  // misc block: barriers | segments | scan scratch | flags
+  // misc block: barriers | segments | flags
   const uint32_t bars = sbase + C::kSmemMisc;
   const uint32_t bar_kfull = bars, bar_kempty = bar_kfull + 8 * kStagesK;
   const uint32_t bar_vfull = bar_kempty + 8 * kStagesK, bar_vempty = bar_vfull + 8 * kStagesV;
   const uint32_t bar_segfull = bar_vempty + 8 * kStagesV, bar_segempty = bar_segfull + 8 * kSegRing;
   const uint32_t bar_x = bar_segempty + 8 * kSegRing;
   const uint32_t bar_qfull = bar_x, bar_qfree = bar_x + 8, bar_s = bar_x + 16, bar_sfree = bar_x + 24, bar_p = bar_x + 32,
-                 bar_pv = bar_x + 40, bar_ofree = bar_x + 48, bar_seg = bar_x + 56, bar_drain = bar_x + 64;
-  constexpr int kBarBytes = 8 * (2 * kStagesK + 2 * kStagesV + 2 * kSegRing + 9);
+                 bar_pv = bar_x + 40, bar_ofree = bar_x + 48, bar_seg = bar_x + 56, bar_drain = bar_x + 64,
+                 bar_join = bar_x + 72;
+  const uint32_t bar_count = bar_x + 80;  // arrival counts ready: one for each of the CTA's (up to) two parts
+  constexpr int kBarBytes = 8 * (2 * kStagesK + 2 * kStagesV + 2 * kSegRing + 12);
   constexpr int kSegOff = (kBarBytes + 15) / 16 * 16;
   uint8_t* misc = smem + C::kSmemMisc;
   Segment* segs = reinterpret_cast<Segment*>(misc + kSegOff);
-  constexpr int kScanOff = kSegOff + kSegRing * static_cast<int>(sizeof(Segment));
-  long long* s_scan = reinterpret_cast<long long*>(misc + kScanOff);  // one per warp
-  struct Start {
-    long long offset, total, s0, s1;
-    int request, used;
-  };
-  Start* start = reinterpret_cast<Start*>(misc + kScanOff + 8 * (kThreads / 32));
-  constexpr int kFlagOff = kScanOff + 8 * (kThreads / 32) + static_cast<int>(sizeof(Start));
+  constexpr int kFlagOff = kSegOff + kSegRing * static_cast<int>(sizeof(Segment));
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + kFlagOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + kFlagOff + 4);
   volatile int* bad_flag = reinterpret_cast<volatile int*>(misc + kFlagOff + 8);
+  volatile int* last_flag = reinterpret_cast<volatile int*>(misc + kFlagOff + 12);
   static_assert(kFlagOff + 16 <= 1024, "misc block");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -282,6 +194,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
     }
     mbar_init(bar_qfull, 1);
     mbar_init(bar_qfree, 1);
+    mbar_init(bar_count, 1);
+    mbar_init(bar_count + 8, 1);
+    mbar_init(bar_join, 4);
     mbar_init(bar_s, 1);
     mbar_init(bar_sfree, 4);  // one arrival per softmax warp
     mbar_init(bar_p, 4);
@@ -291,7 +206,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
     mbar_init(bar_drain, 1);
     *abort_flag = 0;
     *bad_flag = 0;
-    start->request = -1;
     fence_mbar_init();
     tma_prefetch_desc(&p.tm_q);
     tma_prefetch_desc(&p.tm_k);
@@ -302,142 +216,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
     tmem_relinquish();
     tc_fence_before();
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  // ---- this CTA's share: prefix sum of the requests' tiles ----
-  {
-    const int per = (p.requests + kThreads - 1) / kThreads;
-    const int b0 = min(tid * per, p.requests), b1 = min(b0 + per, p.requests);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b)
-      mine += p.kv_heads * head_tiles<kBN>(p, request_of(p, p.cu[b], p.cu[b + 1], p.context[b], cta == 0));
-    long long incl = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += x;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
-    long long before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      const long long x = s_scan[w];
-      if (w < warp) before += x;
-      total += x;
-    }
-    before += incl - mine;
-    const long long most = (total + FL_TREE_MIN_STEPS - 1) / FL_TREE_MIN_STEPS;
-    const int used = static_cast<int>(min(static_cast<long long>(p.grid), most));
-    const long long s0 = cta < used ? cta * total / used : 0, s1 = cta < used ? (cta + 1) * total / used : 0;
-    if (s0 < s1 && before <= s0 && s0 < before + mine) {
-      long long at = before;
-      for (int b = b0; b < b1; ++b) {
-        const long long n = p.kv_heads * head_tiles<kBN>(p, request_of(p, p.cu[b], p.cu[b + 1], p.context[b], false));
-        if (s0 < at + n) {
-          start->request = b;
-          start->offset = s0 - at;
-          break;
-        }
-        at += n;
-      }
-    }
-    if (tid == 0) {
-      start->total = total;
-      start->used = used;
-      start->s0 = s0;
-      start->s1 = s1;
-    }
-  }
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsProducer));
     if (warp == 3) {
       // ======================= scheduler =======================
-      const long long total = start->total;
-      const int used = start->used;
-      long long s = start->s0;
-      const long long s1 = start->s1;
-      int b = start->request;
-      long long off = b >= 0 ? start->offset : 0;
-      int ring = 0;
-      bool ok = true;
-      int4 cut = make_int4(0, 0, 0, 0);  // x: parts after the first (0: no unit is cut here)
-      auto post = [&](const Segment& g) -> bool {
+      Scheduler<kBN> sched(p, cta, lane);
+      for (int ring = 0;; ++ring) {
+        const Segment g = sched.next();
         const int st = ring % kSegRing;
-        if (!wait_all(bar_segempty + 8 * st, ((ring / kSegRing) & 1) ^ 1, abort_flag, p.err)) return false;
+        if (!wait_all(bar_segempty + 8 * st, ((ring / kSegRing) & 1) ^ 1, abort_flag, p.err)) break;
         if (lane == 0) {
           segs[st] = g;
           mbar_arrive(bar_segfull + 8 * st);
         }
         __syncwarp();
-        ++ring;
-        return true;
-      };
-      int base = -64;  // lane l holds request base + l
-      int l_begin = 0, l_end = 0, l_ctx = 0;
-      while (ok && s < s1 && b >= 0 && b < p.requests) {
-        if (b >= base + 32 || b < base) {
-          base = b;
-          const int mine = b + lane;
-          l_begin = mine < p.requests ? p.cu[mine] : 0;
-          l_end = mine < p.requests ? p.cu[mine + 1] : 0;
-          l_ctx = mine < p.requests ? p.context[mine] : 0;
+        if (g.t1 < 0) break;
+        if (g.slot >= 0) {
+          ready_counts(p, g, cta, lane);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_count + 8 * (g.slot & 1));
         }
-        const Request r = request_of(p, __shfl_sync(0xffffffffu, l_begin, b - base),
-                                     __shfl_sync(0xffffffffu, l_end, b - base),
-                                     __shfl_sync(0xffffffffu, l_ctx, b - base), false);
-        int h = 0, i0 = 0;
-        if (off > 0) {  // the first request starts part-way
-          const long long per_head = head_tiles<kBN>(p, r);
-          h = static_cast<int>(off / per_head);
-          off -= h * per_head;
-          while (off >= tiles_of<kBN>(p, r, i0)) {
-            off -= tiles_of<kBN>(p, r, i0);
-            i0 += p.tile_tokens;
-          }
-        }
-        for (; ok && s < s1 && r.count > 0 && h < p.kv_heads; ++h, i0 = 0) {
-          for (; ok && s < s1 && i0 < r.count; i0 += p.tile_tokens) {
-            const int n = tiles_of<kBN>(p, r, i0);
-            Segment g;
-            g.request = b;
-            g.head = h;
-            g.i0 = i0;
-            g.rows = min(p.tile_tokens, r.count - i0) * p.group;
-            g.begin = r.begin;
-            g.count = r.count;
-            g.ctx = r.ctx;
-            g.keys = keys_of(p, r, i0);
-            g.t0 = static_cast<int>(off);
-            g.t1 = static_cast<int>(min(static_cast<long long>(n), off + (s1 - s)));
-            const bool whole = g.t0 == 0 && g.t1 == n;
-            g.slot = whole ? -1 : 2 * cta + (g.t0 == 0 ? 1 : 0);
-            g.pad = 0;
-            if (!whole && g.t0 == 0) {
-              // the unit's first part: the last CTA with tiles of it
-              const long long end = s + n;
-              const int last = static_cast<int>((end * used + total - 1) / total) - 1;
-              cut = make_int4(last - cta, r.begin + i0, h, g.rows);
-            }
-            s += g.t1 - g.t0;
-            off = 0;
-            ok = post(g);
-          }
-        }
-        ++b;
-        off = 0;
       }
-      if (ok) {
-        Segment g = {};
-        g.t1 = -1;
-        post(g);
-      }
-      if (lane == 0) p.cuts[cta] = cut;
     } else if (warp == 0 || warp == 2) {
       // ======================= K (and Q) producer, V producer =======================
       const bool is_k = warp == 0;
@@ -445,7 +250,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       const CUtensorMap* tm = is_k ? &p.tm_k : &p.tm_v;
       const uint32_t ring0 = is_k ? s_k0 : s_v0, full0 = is_k ? bar_kfull : bar_vfull, empty0 = is_k ? bar_kempty : bar_vempty;
       const int page = 1 << p.page_shift;
-      const int boxes = kBN / p.box_rows;  // page boxes per tile
       int tile = 0, seg = 0, q_loads = 0;
       bool ok = true;
       while (ok) {
@@ -456,19 +260,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
         if (lane == 0) mbar_arrive(bar_segempty + 8 * sl);
         ++seg;
         if (g.t1 < 0) break;
-        const int32_t* row = p.table + g.request * p.table_stride;
-        // this lane's box of tile t: its block and first row there
-        auto block_of = [&](int t) -> int {
-          const int key = t * kBN + lane * p.box_rows;
-          if (lane >= boxes || key >= g.keys) return -1;
-          const int blk = row[key >> p.page_shift];
-          if (blk >= 0 && blk < p.num_blocks) return blk;
-          if (is_k) atomicOr(p.err, kDevErrIndex);
-          return p.num_blocks;  // outside the map: zeros arrive, nothing is read
-        };
-        int next = block_of(g.t0);
+        PageNumbers<kBN> pages(p, g, lane);
         if (is_k) {
-          if (!wait_all(bar_qfree, (q_loads & 1) ^ 1, abort_flag, p.err)) break;
+          if (!wait_all(bar_qfree, ((seg - 1) & 1) ^ 1, abort_flag, p.err)) break;
           if (lane == 0) {
             mbar_arrive_expect_tx(bar_qfull, p.group * p.tile_tokens * 128 * C::kHalves);
 #pragma unroll
@@ -479,8 +273,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
           ++q_loads;
         }
         for (int t = g.t0; t < g.t1; ++t, ++tile) {
-          const int blk = next;
-          if (t + 1 < g.t1) next = block_of(t + 1);
+          const int blk = pages.of_tile(g, t, is_k);
           const int st = tile % stages;
           if (!wait_all(empty0 + 8 * st, ((tile / stages) & 1) ^ 1, abort_flag, p.err)) {
             ok = false;
@@ -503,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
         // let every copy this warp started land before shared memory is released
         for (int t = tile > stages ? tile - stages : 0; t < tile; ++t)
           mbar_wait_quiet(full0 + 8 * (t % stages), (t / stages) & 1);
-        if (is_k && q_loads > 0) mbar_wait_quiet(bar_qfull, (q_loads - 1) & 1);
+        if (q_loads > 0) mbar_wait_quiet(bar_qfull, (q_loads - 1) & 1);
       }
     } else {
       // ======================= MMA issuer =======================
@@ -514,6 +307,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       const uint64_t dk0 = make_sdesc_sw128(s_k0, 16, 1024);
       const uint64_t dv0 = make_sdesc_sw128(s_v0, HD == 64 ? 8192 : kBN * 128, 1024);
       constexpr uint64_t kStageEnc = C::kTileBytes >> 4, kQHalf = (kBM * 128) >> 4, kKHalf = (kBN * 128) >> 4;
+      auto ready = [&](uint32_t bar, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, mbar_try_wait_hint(bar, parity, FL_ISSUER_HINT_NS));
+      };
+      // Keeps trying until the step is done; bounded like every wait.
+      auto until = [&](auto&& step) -> bool {
+        if (step()) return true;
+        const uint64_t t0 = globaltimer_ns();
+        while (true) {
+#pragma unroll 1
+          for (int k = 0; k < 64; ++k)
+            if (step()) return true;
+          const bool late = globaltimer_ns() - t0 > FL_WAIT_LIMIT_NS;
+          if (__any_sync(0xffffffffu, late || *abort_flag)) {
+            if (lane == 0 && !*abort_flag) {
+              *abort_flag = 1;
+              if (p.err) atomicOr(p.err, kDevErrWaitTimeout);
+            }
+            return false;
+          }
+        }
+      };
       int ks = 0, vs = 0, seg = 0;  // S products, P V products, segments so far
       bool ok = true;
       while (ok) {
@@ -524,10 +338,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
         if (lane == 0) mbar_arrive(bar_segempty + 8 * sl);
         if (g.t1 < 0) break;
         if (!wait_all_issuer(bar_qfull, seg & 1, abort_flag, p.err)) break;
-        auto issue_s = [&](bool last) -> bool {
+        auto try_s = [&](bool last) -> bool {
           const int st = ks % kStagesK;
-          if (!wait_all_issuer(bar_kfull + 8 * st, (ks / kStagesK) & 1, abort_flag, p.err)) return false;
-          if (!wait_all_issuer(bar_sfree, (ks & 1) ^ 1, abort_flag, p.err)) return false;
+          if (!ready(bar_kfull + 8 * st, (ks / kStagesK) & 1) || !ready(bar_sfree, (ks & 1) ^ 1)) return false;
           tc_fence_after();
           const uint64_t bd = dk0 + st * kStageEnc;
           if (elect_one()) {
@@ -543,35 +356,49 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
           ++ks;
           return true;
         };
-        ok = issue_s(g.t0 + 1 == g.t1);
+        ok = until([&] { return try_s(g.t0 + 1 == g.t1); });
         // O of the segment before has been read
         if (ok) ok = wait_all_issuer(bar_ofree, (seg & 1) ^ 1, abort_flag, p.err);
         if (!ok) break;
         if (lane == 0) *bad_flag = 0;
         // keys from here on are hidden from some row of the tile
         const int mixed = p.mask != nullptr ? g.ctx : min(g.ctx + g.i0 + 1, g.keys);
-        for (int t = g.t0; t < g.t1; ++t) {
-          if (t + 1 < g.t1 && !(ok = issue_s(t + 2 == g.t1))) break;
+        uint32_t accumulate = 0;
+        for (int t = g.t0; ok && t < g.t1; ++t) {
+          // The next S and this tile's P V, in the order in which they can go:
+          // a V tile is not held while the next K tile is awaited.
           const int st = vs % kStagesV;
-          if (!(ok = wait_all_issuer(bar_vfull + 8 * st, (vs / kStagesV) & 1, abort_flag, p.err))) break;
-          const int valid = min(kBN, g.keys - t * kBN), from = max(0, min(mixed - t * kBN, valid));
-          if (from < kBN) {
-            const bool bad = guard_v<T, HD>(s_v0 + st * C::kTileBytes, from, valid, lane);
-            if (bad && lane == 0) *bad_flag = 1;
-            __syncwarp();
-          }
-          if (!(ok = wait_all_issuer(bar_p, vs & 1, abort_flag, p.err))) break;
-          tc_fence_after();
-          const uint64_t bd = dv0 + st * kStageEnc;
-          if (elect_one()) {
+          bool s_done = t + 1 == g.t1, pv_done = false, guarded = false;
+          auto try_pv = [&]() -> bool {
+            if (!guarded) {
+              if (!ready(bar_vfull + 8 * st, (vs / kStagesV) & 1)) return false;
+              const int valid = min(kBN, g.keys - t * kBN), from = max(0, min(mixed - t * kBN, valid));
+              if (from < kBN) {
+                const bool bad = guard_v<T, HD, kBN>(s_v0 + st * C::kTileBytes, from, valid, lane);
+                if (bad && lane == 0) *bad_flag = 1;
+                __syncwarp();
+              }
+              guarded = true;
+            }
+            if (!ready(bar_p, vs & 1)) return false;
+            tc_fence_after();
+            const uint64_t bd = dv0 + st * kStageEnc;
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kBN / 16; ++kk)
-              umma_f16_ts(tm + C::kColO, tm + C::kColP + kk * 8, bd + 128 * kk, idesc_pv,
-                          (kk > 0 || t > g.t0) ? 1u : 0u);
-            umma_commit(bar_pv);
-            umma_commit(bar_vempty + 8 * st);
-          }
-          __syncwarp();
+              for (int kk = 0; kk < kBN / 16; ++kk)
+                umma_f16_ts(tm + C::kColO, tm + C::kColP + kk * 8, bd + 128 * kk, idesc_pv, kk > 0 ? 1u : accumulate);
+              umma_commit(bar_pv);
+              umma_commit(bar_vempty + 8 * st);
+            }
+            __syncwarp();
+            return true;
+          };
+          ok = until([&]() -> bool {
+            if (!s_done) s_done = try_s(t + 2 == g.t1);
+            if (!pv_done) pv_done = try_pv();
+            return s_done && pv_done;
+          });
+          accumulate = 1;
           ++vs;
         }
         if (lane == 0) mbar_arrive(bar_seg);  // publishes bad_flag
@@ -594,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
     const int my_token = t_row / p.group, my_head = t_row % p.group;  // within the row tile
     const float sc = p.scale_log2;
     const bool prescale = !(sc > 0.0f);  // a negative scale turns maxima into minima: applied first
-    int js = 0, seg = 0;                 // tiles and segments so far
+    int js = 0, seg = 0, joins = 0;      // tiles, segments and meetings so far
     bool ok = true;
     while (ok) {
       const int sl = seg % kSegRing;
@@ -742,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
         const float inv = (l > 0.0f) ? 1.0f / norm : 0.0f;
         const float lse2 = (l == 0.0f) ? -INFINITY : (m_ref - kUp) + log2f(l);
         const long long orow = static_cast<long long>(token) * p.heads + g.head * p.group + my_head;
-        float* prow = g.slot < 0 ? nullptr : p.part + (static_cast<long long>(g.slot) * kBM + t_row) * HD;
+        float4* prow = g.slot < 0 ? nullptr : reinterpret_cast<float4*>(p.part) + static_cast<long long>(g.slot) * (HD / 4) * kBM + t_row;
         if (live) {
           if (g.slot >= 0) p.part_lse[g.slot * kBM + t_row] = lse2;
           else if (p.lse != nullptr) p.lse[orow] = lse2 * 0.69314718055994531f;
@@ -778,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
             if (prow != nullptr) {
 #pragma unroll
               for (int c = 0; c < 32; c += 4)
-                *reinterpret_cast<float4*>(prow + 32 * h + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                prow[(8 * h + c / 4) * kBM] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
             } else {
               uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + orow * HD + 32 * h);
 #pragma unroll
@@ -793,16 +620,37 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_ofree);
       ++seg;
+      if (g.slot >= 0) {
+        // a part: whoever arrives last joins, within its group of parts and then among the groups
+        const int first = cta - g.part, groups = (g.parts + kJoinGroup - 1) / kJoinGroup;
+        int base = g.part / kJoinGroup * kJoinGroup, stride = 1, n = min(kJoinGroup, g.parts - base);
+        // the four warps meet with bounded waits: one that has given up does not come
+        auto meet = [&]() -> bool {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_join);
+          return wait_all(bar_join, joins++ & 1, abort_flag, p.err);
+        };
+#pragma unroll 1
+        while (true) {
+          if (!(ok = meet())) break;  // all of this CTA's part is written
+          if (t_row == 0)
+            *last_flag = mbar_wait(bar_count + 8 * (g.slot & 1), 0, abort_flag, p.err) &&
+                         arrive_last(stride == 1 ? group_word(p, g, cta) : unit_word(p, g, cta), n);
+          if (!(ok = meet())) break;
+          if (*last_flag == 0) break;
+          const int to = stride == 1 && groups > 1 ? slot_of(first, base) : -1;
+          const float lse2 = join_parts<T, HD>(p, g, t_row, first, base, stride, n, to);
+          if (to < 0) break;
+          if (!(ok = meet())) break;  // the group's log-sum-exps have been read: its first slot takes the joined ones
+          if (live) p.part_lse[to * kBM + t_row] = lse2;
+          base = 0;
+          stride = kJoinGroup;
+          n = groups;
+        }
+      }
     }
 
-    // rows of q that belong to no request (a batch padded to a fixed size)
-    const int end = p.requests > 0 ? max(0, min(p.cu[p.requests], p.tokens)) : 0;
-    const long long rows = static_cast<long long>(p.tokens - end) * p.heads;
-    for (long long r = static_cast<long long>(cta) * 4 + (warp - 4); r < rows; r += static_cast<long long>(p.grid) * 4) {
-      const long long orow = static_cast<long long>(end) * p.heads + r;
-      if (lane < HD / 8) reinterpret_cast<uint4*>(static_cast<T*>(p.out) + orow * HD)[lane] = make_uint4(0u, 0u, 0u, 0u);
-      if (p.lse != nullptr && lane == 0) p.lse[orow] = -INFINITY;
-    }
+    clear_padding<T, HD>(p, cta * 4 + (warp - 4), p.grid * 4, lane);
   }
 
   __syncthreads();
@@ -812,73 +660,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
   }
 }
 
-// Joins the parts of the units that the division among CTAs cut: part k of
-// the unit that starts in CTA c is slot 2c + 1 (k = 0) or 2(c + k), and
-//   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M),  M = max_k lse_k.
-// A warp per row, lanes across the columns (D = 64: two parts at a time).
-constexpr int kJoinThreads = 256;
-
-template <typename T, int HD>
-__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x;
-  const int4 cut = p.cuts[c];
-  const int parts = cut.x + 1;
-  if (parts <= 1) return;
-  const int lane = threadIdx.x & 31;
-  constexpr int kVecs = HD / 4, kAtOnce = 32 / kVecs;  // float4s per row, parts per pass
-  const int col = lane % kVecs, sub = lane / kVecs;
-  for (int row = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); row < cut.w; row += gridDim.y * (kJoinThreads / 32)) {
-    auto slot = [&](int k) { return k == 0 ? 2 * c + 1 : 2 * (c + k); };
-    float m = -INFINITY;
-    for (int k = lane; k < parts; k += 32) m = fmaxf(m, p.part_lse[slot(k) * kBM + row]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const float m_use = m == -INFINITY ? 0.0f : m;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.0f;
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-      const float w = k0 + lane < parts ? ex2_approx(p.part_lse[slot(k0 + lane) * kBM + row] - m_use) : 0.0f;
-      sum += w;
-      const int here = min(32, parts - k0);
-#pragma unroll 8
-      for (int k = 0; k < here; k += kAtOnce) {
-        const float wk = __shfl_sync(0xffffffffu, w, (k + sub) & 31);
-        if (k + sub < here) {
-          const float4 v = reinterpret_cast<const float4*>(p.part + (static_cast<long long>(slot(k0 + k + sub)) * kBM + row) * HD)[col];
-          acc.x = fmaf(wk, v.x, acc.x);
-          acc.y = fmaf(wk, v.y, acc.y);
-          acc.z = fmaf(wk, v.z, acc.z);
-          acc.w = fmaf(wk, v.w, acc.w);
-        }
-      }
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-#pragma unroll
-    for (int d = 16; d >= kVecs; d >>= 1) {
-      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, d);
-      acc.y += __shfl_xor_sync(0xffffffffu, acc.y, d);
-      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, d);
-      acc.w += __shfl_xor_sync(0xffffffffu, acc.w, d);
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-    const long long orow = static_cast<long long>(cut.y + row / p.group) * p.heads + cut.z * p.group + row % p.group;
-    if (sub == 0)
-      reinterpret_cast<uint2*>(static_cast<T*>(p.out) + orow * HD)[col] =
-          make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-    if (p.lse != nullptr && lane == 0)
-      p.lse[orow] = sum == 0.0f ? -INFINITY : (m_use + log2f(sum)) * 0.69314718055994531f;
-  }
-}
-
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 size_t workspace_bytes(int grid, int64_t head_dim) {
   const size_t slots = 2 * static_cast<size_t>(grid);
-  return slots * kBM * (head_dim + 1) * sizeof(float) + grid * sizeof(int4);
+  return slots * kBM * (head_dim + 1) * sizeof(float) + 3 * grid * sizeof(unsigned long long);
 }
 
 bool encode(CUtensorMap* tm, bool bf16, const void* base, int rank, const cuuint64_t* dims, const int64_t* strides,
@@ -896,28 +683,24 @@ bool encode(CUtensorMap* tm, bool bf16, const void* base, int rank, const cuuint
 
 template <typename T, int HD>
 cudaError_t launch(TreeParams& p, const fl_tree_attention_args& a, cudaStream_t stream) {
-  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int kBN = Shape<HD>::kBN;
-  p.box_rows = static_cast<int>(std::min<int64_t>(a.page_size, kBN));
-  const cuuint64_t dq[3] = {HD, static_cast<cuuint64_t>(a.heads), static_cast<cuuint64_t>(a.tokens)};
-  const cuuint64_t dc[4] = {HD, static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(a.kv_heads),
-                            static_cast<cuuint64_t>(a.num_blocks)};
-  const int64_t sq[2] = {a.q_stride[1], a.q_stride[0]};
-  const int64_t sk[3] = {a.k_stride[1], a.k_stride[2], a.k_stride[0]}, sv[3] = {a.v_stride[1], a.v_stride[2], a.v_stride[0]};
-  const cuuint32_t bq[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(p.tile_tokens)};
-  const cuuint32_t bc[4] = {64, static_cast<cuuint32_t>(p.box_rows), 1, 1};
-  if (!encode(&p.tm_q, bf16, a.q, 3, dq, sq, bq) || !encode(&p.tm_k, bf16, a.k_cache, 4, dc, sk, bc) ||
-      !encode(&p.tm_v, bf16, a.v_cache, 4, dc, sv, bc))
-    return cudaErrorInvalidValue;
+  p.grid = kCtasPerSm * sm_count();
+  p.tile_tokens = kBM / p.group;
+  p.part_lse = p.part + 2LL * p.grid * kBM * HD;
+  p.arrived = reinterpret_cast<unsigned long long*>(p.part_lse + 2LL * p.grid * kBM);
+  if (!encode_tree_maps(p, a, Shape<HD>::kBN)) return cudaErrorInvalidValue;
   auto kern = tree_attention_kernel<T, HD>;
   static std::atomic<bool> configured[kMaxFlagDevices];
-  cudaError_t e = ensure_smem_limit(kern, Shape<HD>::kSmemBytes, configured);
+  const cudaError_t e = ensure_smem_limit(kern, Shape<HD>::kSmemBytes, configured);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, p.grid, kThreads, Shape<HD>::kSmemBytes, stream, p);
-  if (e != cudaSuccess) return e;
-  const int64_t rows = std::min<int64_t>(kBM, a.tokens * p.group);
-  const int ys = static_cast<int>(std::min<int64_t>(4, (rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32)));
-  return launch_pdl(tree_join_kernel<T, HD>, dim3(p.grid, ys), kJoinThreads, 0, stream, p);
+  return launch_pdl(kern, p.grid, kThreads, Shape<HD>::kSmemBytes, stream, p);
+}
+
+// A tag that no earlier call of this process had (the counter goes through
+// 48 bits before it repeats), spread so that what other data leave in the
+// workspace is unlikely to look like one.
+unsigned long long next_tag() {
+  static std::atomic<unsigned long long> calls{0};
+  return ((calls.fetch_add(1, std::memory_order_relaxed) + 1) * 0x9E3779B97F4A7C15ull) & 0xffffffffffffull;
 }
 
 int tree_attention(const fl_tree_attention_args* args, void* stream) {
@@ -954,8 +737,7 @@ int tree_attention(const fl_tree_attention_args* args, void* stream) {
   int st = check_device();
   if (st != FL_OK) return st;
   TreeParams p = {};
-  p.grid = kCtasPerSm * sm_count();
-  if (!a.workspace || a.workspace_bytes < workspace_bytes(p.grid, a.head_dim))
+  if (!a.workspace || a.workspace_bytes < workspace_bytes(kCtasPerSm * sm_count(), a.head_dim))
     return fail(FL_ERR_INVALID_ARGUMENT, "workspace too small (fl_tree_attention_workspace_size)");
   p.v = a.v_cache;
   p.out = a.out;
@@ -965,8 +747,7 @@ int tree_attention(const fl_tree_attention_args* args, void* stream) {
   p.cu = a.cu_seqlens;
   p.mask = a.tree_mask != nullptr && a.mask_words > 0 ? a.tree_mask : nullptr;
   p.part = static_cast<float*>(a.workspace);
-  p.part_lse = p.part + 2LL * p.grid * kBM * a.head_dim;
-  p.cuts = reinterpret_cast<int4*>(p.part_lse + 2LL * p.grid * kBM);
+  p.tag = next_tag();
   p.err = device_error_word();
   for (int i = 0; i < 3; ++i) p.v_stride[i] = a.v_stride[i];
   p.table_stride = a.table_stride;
@@ -975,7 +756,6 @@ int tree_attention(const fl_tree_attention_args* args, void* stream) {
   p.heads = static_cast<int>(a.heads);
   p.kv_heads = static_cast<int>(a.kv_heads);
   p.group = p.heads / p.kv_heads;
-  p.tile_tokens = kBM / p.group;
   while ((1LL << p.page_shift) < a.page_size) ++p.page_shift;
   p.num_blocks = static_cast<int>(a.num_blocks);
   p.table_cols = static_cast<int>(a.table_cols);
@@ -991,6 +771,22 @@ int tree_attention(const fl_tree_attention_args* args, void* stream) {
 }
 
 }  // namespace
+
+bool encode_tree_maps(TreeParams& p, const fl_tree_attention_args& a, int tile_keys) {
+  const bool bf16 = a.dtype == FL_DTYPE_BF16;
+  p.box_rows = static_cast<int>(std::min<int64_t>(a.page_size, tile_keys));
+  const cuuint64_t dq[3] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.heads),
+                            static_cast<cuuint64_t>(a.tokens)};
+  const cuuint64_t dc[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.page_size),
+                            static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.num_blocks)};
+  const int64_t sq[2] = {a.q_stride[1], a.q_stride[0]};
+  const int64_t sk[3] = {a.k_stride[1], a.k_stride[2], a.k_stride[0]}, sv[3] = {a.v_stride[1], a.v_stride[2], a.v_stride[0]};
+  const cuuint32_t bq[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(p.tile_tokens)};
+  const cuuint32_t bc[4] = {64, static_cast<cuuint32_t>(p.box_rows), 1, 1};
+  return encode(&p.tm_q, bf16, a.q, 3, dq, sq, bq) && encode(&p.tm_k, bf16, a.k_cache, 4, dc, sk, bc) &&
+         encode(&p.tm_v, bf16, a.v_cache, 4, dc, sv, bc);
+}
+
 }  // namespace fl
 
 extern "C" size_t fl_tree_attention_workspace_size(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {

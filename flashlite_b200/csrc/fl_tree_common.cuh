@@ -1,0 +1,409 @@
+// Shared by the kernels of attention over a paged cache (fl_tree.cu: up to 128
+// rows a unit; fl_tree_few.cu: few rows): launch parameters, the division of
+// the work, the joining of cut units and the guard of V tiles.
+//
+// A unit of work is (request, key head, row tile): as many of the request's
+// tokens as fill a tile's rows, each with the query heads that share the key
+// head, so that a key and value is read once for all of them. A unit's keys
+// are cut into tiles; all tiles of all units, laid end to end, are divided
+// evenly among the CTAs whatever the requests' lengths, which are read on the
+// device. A CTA that ends up with part of a unit leaves an fp32 partial
+// result, and whichever CTA finishes a cut unit last joins its parts, in their
+// order whoever that is (the same bits every time), and nobody waits for
+// anyone.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/flashlite_b200.h"
+#include "fl_internal.h"
+#include "fl_ptx.cuh"
+#include "fl_types.cuh"
+
+namespace fl {
+
+struct TreeParams {
+  CUtensorMap tm_q;  // {D, heads, tokens}, box {64, group, tile_tokens}
+  CUtensorMap tm_k;  // {D, page rows, key heads, blocks}, box {64, box_rows, 1, 1}
+  CUtensorMap tm_v;
+  const void* v;
+  void* out;
+  float* lse;
+  const int32_t* table;
+  const int32_t* context;
+  const int32_t* cu;
+  const uint32_t* mask;
+  float* part;      // partial results, 2 * grid slots: CTA c's are 2c (a unit's later part) and 2c + 1 (its first)
+  float* part_lse;  // their log2-sum-exp, a tile's rows for each slot
+  unsigned long long* arrived;  // [2 * grid] by group of parts, [grid] by unit: tag and count
+  unsigned long long tag;       // 48 bits, another one for each call
+  unsigned int* err;
+  long long v_stride[3];
+  long long table_stride;
+  int requests, tokens, heads, kv_heads, group, tile_tokens;
+  int page_shift, box_rows, num_blocks, table_cols, mask_words;
+  float scale_log2;
+  int grid;
+};
+
+// Attention of few rows (fl_tree_few.cu): rows 16 or 32 to a unit. The caller
+// has filled in everything but what depends on the kernel's tiles.
+cudaError_t launch_tree_few(TreeParams& p, const fl_tree_attention_args& a, int rows, cudaStream_t stream);
+// Tensor maps of q, the caches for tiles of kBN keys and row tiles of p.tile_tokens.
+bool encode_tree_maps(TreeParams& p, const fl_tree_attention_args& a, int tile_keys);
+
+namespace {
+
+constexpr int kSegRing = 4;  // work descriptors between the scheduler and the other warps
+
+// A reference maximum is kept until a row's maximum exceeds it by this much
+// (log2); probabilities are held 2^kUp times their size, so that fp16 keeps
+// the small ones out of its subnormal range: at most 2^15 after the lag.
+constexpr float kLag = 8.0f, kUp = 7.0f;
+
+// One request as the schedule sees it.
+struct Request {
+  int begin, count, ctx, room;  // first row of q, new tokens, cached tokens, keys its table row can name
+};
+
+__device__ __forceinline__ Request request_of(const TreeParams& p, int begin, int end, int ctx, bool report) {
+  Request r;
+  const long long room = static_cast<long long>(p.table_cols) << p.page_shift;
+  r.room = room > 0x3fffffff ? 0x3fffffff : static_cast<int>(room);
+  bool sound = true;
+  r.begin = begin;
+  r.count = end - begin;
+  if (begin < 0 || end < begin || end > p.tokens) {
+    sound = false;
+    r.begin = r.count = 0;
+  }
+  r.ctx = ctx;
+  if (ctx < 0 || ctx > r.room) {
+    sound = false;
+    r.ctx = ctx < 0 ? 0 : r.room;
+  }
+  if (r.count > r.room - r.ctx) sound = false;  // the new tokens past the table's end are not visible
+  if (!sound && report) atomicOr(p.err, kDevErrIndex);
+  return r;
+}
+
+// Keys that some row of the row tile with tokens [i0, i0 + n) may see.
+__device__ __forceinline__ int keys_of(const TreeParams& p, const Request& r, int i0) {
+  int inner;
+  if (p.mask != nullptr) inner = min(r.count, 32 * p.mask_words);
+  else inner = min(r.count, i0 + p.tile_tokens);
+  return min(r.ctx + inner, r.room);
+}
+
+template <int kBN>
+__device__ __forceinline__ int tiles_of(const TreeParams& p, const Request& r, int i0) {
+  return max(1, (keys_of(p, r, i0) + kBN - 1) / kBN);
+}
+
+// Tiles of one key head of a request: those of all its row tiles.
+template <int kBN>
+__device__ __forceinline__ long long head_tiles(const TreeParams& p, const Request& r) {
+  if (r.count == 0) return 0;
+  if (p.mask != nullptr)
+    return static_cast<long long>((r.count + p.tile_tokens - 1) / p.tile_tokens) * tiles_of<kBN>(p, r, 0);
+  long long n = 0;
+  for (int i0 = 0; i0 < r.count; i0 += p.tile_tokens) n += tiles_of<kBN>(p, r, i0);
+  return n;
+}
+
+__device__ __forceinline__ long long divide(long long a, long long b) {  // a, b >= 0
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// The division of `total` tiles among `used` CTAs: CTA c begins with tile
+// floor(c total / used), so that tile u is the share of CTA
+// ceil((u + 1) used / total) - 1.
+struct Division {
+  long long total;
+  int used;
+  __device__ __forceinline__ long long begin(int c) const { return divide(c * total, used); }
+  __device__ __forceinline__ int owner(long long u) const { return static_cast<int>(divide((u + 1) * used - 1, total)); }
+};
+
+// A CTA's share of one unit: tiles [t0, t1) of n.
+struct Segment {
+  int request, head, i0, rows;  // rows = tokens in the row tile times group
+  int begin, count, ctx, keys;
+  int t0, t1;                   // t1 < 0: no more work
+  int slot;                     // partial result, -1: the whole unit, written to out
+  int part, parts;              // which of the unit's how many parts
+};
+
+
+// The scheduler of one CTA: a warp that walks over the CTA's share of the
+// tiles and hands out its segments. All lanes hold the same state, but for the
+// 32 requests from `base` on, one a lane.
+template <int kBN>
+struct Scheduler {
+  const TreeParams& p;
+  const int cta, lane;
+  Division div;
+  long long s, s1, off;  // next tile, end of the share, tiles of the current request before s
+  int b, h, i0;          // request, key head, first token of the row tile
+  bool entered;          // whether h and i0 are those of request b
+  int base, l_begin, l_end, l_ctx;
+  Request r;
+
+  __device__ __forceinline__ Scheduler(const TreeParams& p_, int cta_, int lane_) : p(p_), cta(cta_), lane(lane_) {
+    load(0);
+    const int per = (p.requests + 31) / 32;  // each lane sums a run of requests
+    const int b0 = min(lane * per, p.requests), b1 = min(b0 + per, p.requests);
+    long long mine = 0;
+    if (per <= 1) {
+      if (lane < p.requests) mine = p.kv_heads * head_tiles<kBN>(p, request_of(p, l_begin, l_end, l_ctx, cta == 0));
+    } else {
+      for (int x = b0; x < b1; ++x) mine += tiles(x, cta == 0);
+    }
+    long long before = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, before, d);
+      if (lane >= d) before += x;
+    }
+    div.total = __shfl_sync(0xffffffffu, before, 31);
+    div.used = static_cast<int>(min(static_cast<long long>(p.grid), div.total));
+    before -= mine;
+    s = s1 = off = 0;
+    b = h = i0 = 0;
+    entered = false;
+    if (cta >= div.used) return;
+    s = div.begin(cta);
+    s1 = div.begin(cta + 1);
+    const bool here = before <= s && s < before + mine;  // the share begins in this lane's run
+    if (here) {
+      b = b0;
+      if (per > 1) {
+        for (long long n = tiles(b, false); s >= before + n; n = tiles(b, false)) {
+          before += n;
+          ++b;
+        }
+      }
+      off = s - before;
+    }
+    const int owner = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    b = __shfl_sync(0xffffffffu, b, owner);
+    off = __shfl_sync(0xffffffffu, off, owner);
+  }
+
+  // The next segment, or t1 = -1 after the last.
+  __device__ __forceinline__ Segment next() {
+    Segment g = {};
+    g.t1 = -1;
+    if (s >= s1) return g;
+    while (true) {
+      if (!entered) {
+        if (b >= p.requests) return g;
+        if (b >= base + 32) load(b);
+        r = request_of(p, __shfl_sync(0xffffffffu, l_begin, b - base), __shfl_sync(0xffffffffu, l_end, b - base),
+                       __shfl_sync(0xffffffffu, l_ctx, b - base), false);
+        h = i0 = 0;
+        if (off > 0) {  // the share begins inside this request
+          const long long per_head = head_tiles<kBN>(p, r);
+          h = static_cast<int>(divide(off, per_head));
+          off -= h * per_head;
+          while (off >= tiles_of<kBN>(p, r, i0)) {
+            off -= tiles_of<kBN>(p, r, i0);
+            i0 += p.tile_tokens;
+          }
+        }
+        entered = true;
+      }
+      if (i0 >= r.count) {
+        i0 = 0;
+        ++h;
+      }
+      if (r.count > 0 && h < p.kv_heads) break;
+      ++b;
+      off = 0;
+      entered = false;
+    }
+    const int n = tiles_of<kBN>(p, r, i0);
+    g.request = b;
+    g.head = h;
+    g.i0 = i0;
+    g.rows = min(p.tile_tokens, r.count - i0) * p.group;
+    g.begin = r.begin;
+    g.count = r.count;
+    g.ctx = r.ctx;
+    g.keys = keys_of(p, r, i0);
+    g.t0 = static_cast<int>(off);
+    g.t1 = static_cast<int>(min(static_cast<long long>(n), off + (s1 - s)));
+    const bool whole = g.t0 == 0 && g.t1 == n;
+    g.slot = whole ? -1 : 2 * cta + (g.t0 == 0 ? 1 : 0);
+    g.part = 0;
+    g.parts = 1;
+    if (!whole) {
+      const int first = div.owner(s - off);
+      g.part = cta - first;
+      g.parts = div.owner(s - off + n - 1) - first + 1;
+    }
+    s += g.t1 - g.t0;
+    off = 0;
+    i0 += p.tile_tokens;
+    return g;
+  }
+
+ private:
+  __device__ __forceinline__ void load(int from) {
+    base = from;
+    const int x = from + lane;
+    l_begin = l_end = l_ctx = 0;
+    if (x < p.requests) {
+      l_begin = p.cu[x];
+      l_end = p.cu[x + 1];
+      l_ctx = p.context[x];
+    }
+  }
+  __device__ __forceinline__ long long tiles(int x, bool report) const {
+    return p.kv_heads * head_tiles<kBN>(p, request_of(p, p.cu[x], p.cu[x + 1], p.context[x], report));
+  }
+};
+
+// Block numbers of a segment's pages, for a producer warp: 32 at a time, one a
+// lane, and the next 32 already under way. (Read one tile ahead, they arrived
+// too late once the memory was busy: 3,000 cycles a tile where the tile itself
+// needed 1,500.)
+template <int kBN>
+struct PageNumbers {
+  const TreeParams& p;
+  const int32_t* row;
+  int base, last, cur, next, lane;
+
+  __device__ __forceinline__ PageNumbers(const TreeParams& p_, const Segment& g, int lane_) : p(p_), lane(lane_) {
+    row = p.table + g.request * p.table_stride;
+    base = g.t0 * kBN >> p.page_shift;
+    last = (min(g.t1 * kBN, g.keys) - 1) >> p.page_shift;  // -1: no key at all
+    cur = load(base + lane);
+    next = load(base + 32 + lane);
+  }
+  // The block of this lane's box of tile t; -1: no box, num_blocks (outside
+  // the map: zeros arrive and nothing is read) for a number out of range.
+  __device__ __forceinline__ int of_tile(const Segment& g, int t, bool report) {
+    if ((t * kBN >> p.page_shift) - base >= 32) {
+      cur = next;
+      base += 32;
+      next = load(base + 32 + lane);
+    }
+    const int key = t * kBN + lane * p.box_rows;
+    const int blk = __shfl_sync(0xffffffffu, cur, (key >> p.page_shift) - base);
+    if (lane >= kBN / p.box_rows || key >= g.keys) return -1;
+    if (blk >= 0 && blk < p.num_blocks) return blk;
+    if (report) atomicOr(p.err, kDevErrIndex);
+    return p.num_blocks;
+  }
+
+ private:
+  __device__ __forceinline__ int load(int page) const { return page <= last ? row[page] : 0; }
+};
+
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err));
+}
+__device__ __forceinline__ bool wait_all_issuer(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                                unsigned int* err) {
+  return __all_sync(0xffffffffu, mbar_wait_issuer(bar, parity, abort_flag, err));
+}
+
+// Exponent bits of the type, all set in infinities and NaN.
+template <typename T>
+constexpr uint32_t kExpBits = 0x7C00u;
+template <>
+constexpr uint32_t kExpBits<__nv_bfloat16> = 0x7F80u;
+
+// A pair with its infinite and NaN elements cleared.
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  constexpr uint32_t e = kExpBits<T>;
+  if ((w & e) == e) w &= 0xffff0000u;
+  if ((w >> 16 & e) == e) w &= 0x0000ffffu;
+  return w;
+}
+
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Makes a V tile of [kBN][HD] (64-column halves side by side) safe for the
+// product, by one warp: rows [valid, kBN) cleared, infinities and NaN in rows
+// [mixed, valid) cleared. Returns whether any were.
+template <typename T, int HD, int kBN>
+__device__ __forceinline__ bool guard_v(uint32_t tile, int mixed, int valid, int lane) {
+  bool bad = false;
+#pragma unroll
+  for (int hh = 0; hh < HD / 64; ++hh) {
+    const uint32_t half = tile + hh * (kBN * 128);
+    for (int c = valid * 8 + lane; c < kBN * 8; c += 32) st_shared_v4(half + c * 16, 0u, 0u, 0u, 0u);
+    for (int c = mixed * 8 + lane; c < valid * 8; c += 32) {
+      const uint4 v = ld_shared_v4(half + c * 16);
+      const uint4 f = make_uint4(finite2<T>(v.x), finite2<T>(v.y), finite2<T>(v.z), finite2<T>(v.w));
+      if (f.x != v.x || f.y != v.y || f.z != v.z || f.w != v.w) {
+        st_shared_v4(half + c * 16, f.x, f.y, f.z, f.w);
+        bad = true;
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  return __any_sync(0xffffffffu, bad);
+}
+
+// Parts are joined in groups of this many, and the groups' results once more:
+// up to 18 x 18 parts, one for each CTA, and no CTA reads more than 18 at once.
+constexpr int kJoinGroup = 18;
+
+// Arrivals are counted in 64-bit words of the workspace: the call's tag above
+// a 16-bit count. The memory needs no clearing: before its part is begun each
+// CTA turns a word with another tag, whatever an earlier use left there, into
+// this call's with a count of zero (one of them succeeds, and none can after
+// the first arrival). The last arrival clears the word, for a captured call
+// that runs again with the same tag.
+__device__ __forceinline__ int slot_of(int first, int part) { return part == 0 ? 2 * first + 1 : 2 * (first + part); }
+__device__ __forceinline__ unsigned long long* group_word(const TreeParams& p, const Segment& g, int cta) {
+  return p.arrived + slot_of(cta - g.part, g.part / kJoinGroup * kJoinGroup);
+}
+__device__ __forceinline__ unsigned long long* unit_word(const TreeParams& p, const Segment& g, int cta) {
+  return p.arrived + 2 * p.grid + (cta - g.part);
+}
+// By the first two lanes of the scheduler warp, for a part g of CTA cta.
+__device__ __forceinline__ void ready_counts(const TreeParams& p, const Segment& g, int cta, int lane) {
+  if (lane >= 2) return;
+  unsigned long long* word = lane == 0 ? group_word(p, g, cta) : unit_word(p, g, cta);
+  const unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(word);
+  if ((seen >> 16) != p.tag) atomicCAS(word, seen, p.tag << 16);
+}
+__device__ __forceinline__ bool arrive_last(unsigned long long* word, int n) {
+  unsigned long long old;
+  asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], 1;" : "=l"(old) : "l"(word) : "memory");
+  if (static_cast<int>(old & 0xffffu) + 1 != n) return false;
+  *reinterpret_cast<volatile unsigned long long*>(word) = 0ull;
+  return true;
+}
+
+// Rows of q that belong to no request (a batch padded to a fixed size): by
+// warp `worker` of `workers`.
+template <typename T, int HD>
+__device__ __forceinline__ void clear_padding(const TreeParams& p, int worker, int workers, int lane) {
+  const int end = p.requests > 0 ? max(0, min(p.cu[p.requests], p.tokens)) : 0;
+  const long long rows = static_cast<long long>(p.tokens - end) * p.heads;
+  for (long long r = worker; r < rows; r += workers) {
+    const long long orow = static_cast<long long>(end) * p.heads + r;
+    if (lane < HD / 8) reinterpret_cast<uint4*>(static_cast<T*>(p.out) + orow * HD)[lane] = make_uint4(0u, 0u, 0u, 0u);
+    if (p.lse != nullptr && lane == 0) p.lse[orow] = -INFINITY;
+  }
+}
+
+}  // namespace
+}  // namespace fl
