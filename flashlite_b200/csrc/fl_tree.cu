@@ -37,6 +37,10 @@ constexpr int kMaxRequests = 4096;
 constexpr uint32_t kTmemCols = 256;
 constexpr int kSegReaders = 7;     // K, V, MMA and four softmax warps
 constexpr int kCtasPerSm = 2;
+// Units of more rows look before they write a part whether they are the last
+// (tree of 61 nodes x 4 heads: 99 -> 89 us); with few rows the look costs more
+// than the part (3 us on the smallest calls).
+constexpr int kDirectRows = 32;
 
 // Shape per head dimension; tiles are made of 64-column (128-byte) swizzle
 // atoms as in the other forward kernels. K and V tiles are 16 KB both ways;
@@ -60,8 +64,44 @@ struct Shape {
   static_assert(kColP + kBN / 2 <= kTmemCols, "TMEM");
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
 };
-// Register split: 128 x 64 (producers, MMA, scheduler) + 128 x 192 (softmax) = 256 x 128, the launch's total.
-constexpr int kRegsProducer = 64, kRegsSoftmax = 192;
+// Register split between the producer, MMA and scheduler warps and the softmax
+// warps, whose row of scores is 128 registers at head dimension 64 and 64 at
+// 128: 128 * (72 + 184) = 128 * (88 + 168) = 256 * 128, the launch's total.
+// (64 + 192 spilled in the MMA warp: tree 98 us for 87, chunk 303 for 282.)
+template <int HD>
+constexpr int kRegsProducer = HD == 64 ? 72 : 88;
+template <int HD>
+constexpr int kRegsSoftmax = 256 - kRegsProducer<HD>;
+
+// One step of a join, a running maximum over parts taken two (or more) at a
+// time: acc, sum and m take in parts with log2-sum-exps l and values v.
+template <int kBatch, int kVals>
+__device__ __forceinline__ void join_step(float& m, float& sum, float (&acc)[kVals], const float (&l)[kBatch],
+                                          const float (&v)[kBatch][kVals]) {
+  float m_new = m;
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, l[k]);
+  const float m_use = m_new == -INFINITY ? 0.0f : m_new, alpha = ex2_approx(m - m_use);
+  m = m_new;
+  sum *= alpha;
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) acc[j] *= alpha;
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k) {
+    const float w = ex2_approx(l[k] - m_use);
+    sum += w;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) acc[j] = fmaf(w, v[k][j], acc[j]);
+  }
+}
+__device__ __forceinline__ float join_inv(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+__device__ __forceinline__ float join_lse(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
+__device__ __forceinline__ void get4(float* to, const float4& v) {
+  to[0] = v.x;
+  to[1] = v.y;
+  to[2] = v.z;
+  to[3] = v.w;
+}
 
 // Joins the n partial results base, base + stride, ... of a unit:
 //   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M),  M = max_k lse_k,
@@ -81,21 +121,19 @@ __device__ __forceinline__ float join_parts(const TreeParams& p, const Segment& 
   const int token = g.begin + g.i0 + row / p.group, head = g.head * p.group + row % p.group;
   const long long orow = static_cast<long long>(token) * p.heads + head;
   float lse2 = 0.0f;
-  // kCols columns of kBatch parts at a time, all their loads under way
-  // together; M is a running maximum. Rolled otherwise: on its first run in a
-  // kernel, code costs as much to fetch as to execute.
+  // kCols columns (of four) of kBatch parts at a time, all their loads under
+  // way together. Rolled otherwise: on its first run in a kernel, code costs
+  // as much to fetch as to execute.
   auto join = [&](auto cols, auto batch) {
     constexpr int kCols = decltype(cols)::value, kBatch = decltype(batch)::value;
 #pragma unroll 1
     for (int c = c0; c < kVecs; c += kCols * lanes) {
-      float4 acc[kCols];
-      float m = -INFINITY, sum = 0.0f;
+      float acc[4 * kCols], m = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int j = 0; j < 4 * kCols; ++j) acc[j] = 0.0f;
 #pragma unroll 1
       for (int k0 = 0; k0 < n; k0 += kBatch) {
-        float l[kBatch];
-        float4 v[kBatch][kCols];
+        float l[kBatch], v[kBatch][4 * kCols];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const bool in = k0 + k < n;
@@ -104,33 +142,17 @@ __device__ __forceinline__ float join_parts(const TreeParams& p, const Segment& 
           const float4* from = reinterpret_cast<const float4*>(p.part) + static_cast<long long>(sl) * kVecs * kBM + row;
 #pragma unroll
           for (int j = 0; j < kCols; ++j)
-            v[k][j] = in && c + j * lanes < kVecs ? __ldcg(from + (c + j * lanes) * kBM) : make_float4(0.f, 0.f, 0.f, 0.f);
+            get4(v[k] + 4 * j, in && c + j * lanes < kVecs ? __ldcg(from + (c + j * lanes) * kBM)
+                                                           : make_float4(0.f, 0.f, 0.f, 0.f));
         }
-        float m_new = m;
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, l[k]);
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new, alpha = ex2_approx(m - m_use);
-        m = m_new;
-        sum *= alpha;
-#pragma unroll
-        for (int j = 0; j < kCols; ++j)
-          acc[j] = make_float4(acc[j].x * alpha, acc[j].y * alpha, acc[j].z * alpha, acc[j].w * alpha);
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const float w = ex2_approx(l[k] - m_use);
-          sum += w;
-#pragma unroll
-          for (int j = 0; j < kCols; ++j)
-            acc[j] = make_float4(fmaf(w, v[k][j].x, acc[j].x), fmaf(w, v[k][j].y, acc[j].y), fmaf(w, v[k][j].z, acc[j].z),
-                                 fmaf(w, v[k][j].w, acc[j].w));
-        }
+        join_step<kBatch, 4 * kCols>(m, sum, acc, l, v);
       }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
+      const float inv = join_inv(sum);
+      lse2 = join_lse(m, sum);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) {
         if (c + j * lanes >= kVecs) break;
-        const float4 o = make_float4(acc[j].x * inv, acc[j].y * inv, acc[j].z * inv, acc[j].w * inv);
+        const float4 o = make_float4(acc[4 * j] * inv, acc[4 * j + 1] * inv, acc[4 * j + 2] * inv, acc[4 * j + 3] * inv);
         if (to >= 0)
           reinterpret_cast<float4*>(p.part)[(static_cast<long long>(to) * kVecs + c + j * lanes) * kBM + row] = o;
         else
@@ -139,6 +161,7 @@ __device__ __forceinline__ float join_parts(const TreeParams& p, const Segment& 
       }
     }
   };
+  static_assert(kDirectRows >= 32, "units that are joined from registers take the first form");
   if (lanes * 4 <= kVecs) join(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
   else join(std::integral_constant<int, 1>{}, std::integral_constant<int, 6>{});
   if (c0 == 0 && to < 0 && p.lse != nullptr) p.lse[orow] = lse2 * 0.69314718055994531f;
@@ -223,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsProducer));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsProducer<HD>));
     if (warp == 3) {
       // ======================= scheduler =======================
       Scheduler<kBN> sched(p, cta, lane);
@@ -413,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsSoftmax<HD>));
     // ======================= softmax: one thread per row =======================
     const int t_row = tid - 128;
     const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
@@ -423,6 +446,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
     const bool prescale = !(sc > 0.0f);  // a negative scale turns maxima into minima: applied first
     int js = 0, seg = 0, joins = 0;      // tiles, segments and meetings so far
     bool ok = true;
+    // the four warps meet with bounded waits: one that has given up does not come
+    auto meet = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_join);
+      return wait_all(bar_join, joins++ & 1, abort_flag, p.err);
+    };
     while (ok) {
       const int sl = seg % kSegRing;
       if (!wait_all(bar_segfull + 8 * sl, (seg / kSegRing) & 1, abort_flag, p.err)) break;
@@ -559,6 +588,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       }
       if (!ok) break;
 
+      // A part whose unit's other parts are all there already is joined from
+      // its registers and never written: as a rule a unit's later part ends
+      // while the CTA of its first part is still at work.
+      const int first = cta - g.part;
+      bool direct = false;
+      if (g.slot >= 0 && g.parts <= kJoinGroup && g.rows > kDirectRows) {
+        if (t_row == 0)
+          *last_flag = mbar_wait(bar_count + 8 * (g.slot & 1), 0, abort_flag, p.err) &&
+                       others_arrived(group_word(p, g, cta), p.tag, g.parts);
+        if (!(ok = meet())) break;
+        direct = *last_flag != 0;
+      }
+
       // ---- epilogue of the segment ----
       if (!(ok = wait_all(bar_pv, (js - 1) & 1, abort_flag, p.err))) break;
       if (!(ok = wait_all(bar_seg, seg & 1, abort_flag, p.err))) break;
@@ -569,10 +611,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
         const float inv = (l > 0.0f) ? 1.0f / norm : 0.0f;
         const float lse2 = (l == 0.0f) ? -INFINITY : (m_ref - kUp) + log2f(l);
         const long long orow = static_cast<long long>(token) * p.heads + g.head * p.group + my_head;
-        float4* prow = g.slot < 0 ? nullptr : reinterpret_cast<float4*>(p.part) + static_cast<long long>(g.slot) * (HD / 4) * kBM + t_row;
+        float4* prow = g.slot < 0 || direct
+                           ? nullptr
+                           : reinterpret_cast<float4*>(p.part) + static_cast<long long>(g.slot) * (HD / 4) * kBM + t_row;
         if (live) {
-          if (g.slot >= 0) p.part_lse[g.slot * kBM + t_row] = lse2;
-          else if (p.lse != nullptr) p.lse[orow] = lse2 * 0.69314718055994531f;
+          if (prow != nullptr) p.part_lse[g.slot * kBM + t_row] = lse2;
+          else if (!direct && p.lse != nullptr) p.lse[orow] = lse2 * 0.69314718055994531f;
         }
 #pragma unroll 1
         for (int h = 0; h < HD / 32; ++h) {
@@ -601,6 +645,34 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
               }
             }
           }
+          if (direct && live) {
+            // as join_parts does it, with this part from its registers
+            float acc[32], m = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) acc[c] = 0.0f;
+#pragma unroll 1
+            for (int k0 = 0; k0 < g.parts; k0 += 2) {
+              float l2[2], v[2][32];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const bool in = k0 + k < g.parts, mine = k0 + k == g.part;
+                const int sl = slot_of(first, min(k0 + k, g.parts - 1));
+                l2[k] = !in ? -INFINITY : mine ? lse2 : __ldcg(p.part_lse + sl * kBM + t_row);
+                const float4* from = reinterpret_cast<const float4*>(p.part) +
+                                     (static_cast<long long>(sl) * (HD / 4) + 8 * h) * kBM + t_row;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                  get4(v[k] + 4 * c, in && !mine ? __ldcg(from + c * kBM) : make_float4(0.f, 0.f, 0.f, 0.f));
+#pragma unroll
+                for (int c = 0; c < 32; ++c) v[k][c] = mine ? o[c] : v[k][c];
+              }
+              join_step<2, 32>(m, sum, acc, l2, v);
+            }
+            const float joined = join_inv(sum);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = acc[c] * joined;
+            if (h == 0 && p.lse != nullptr) p.lse[orow] = join_lse(m, sum) * 0.69314718055994531f;
+          }
           if (live) {
             if (prow != nullptr) {
 #pragma unroll
@@ -620,16 +692,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_ofree);
       ++seg;
-      if (g.slot >= 0) {
+      if (g.slot >= 0 && !direct) {
         // a part: whoever arrives last joins, within its group of parts and then among the groups
-        const int first = cta - g.part, groups = (g.parts + kJoinGroup - 1) / kJoinGroup;
+        const int groups = (g.parts + kJoinGroup - 1) / kJoinGroup;
         int base = g.part / kJoinGroup * kJoinGroup, stride = 1, n = min(kJoinGroup, g.parts - base);
-        // the four warps meet with bounded waits: one that has given up does not come
-        auto meet = [&]() -> bool {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_join);
-          return wait_all(bar_join, joins++ & 1, abort_flag, p.err);
-        };
 #pragma unroll 1
         while (true) {
           if (!(ok = meet())) break;  // all of this CTA's part is written

@@ -95,9 +95,7 @@ __device__ __forceinline__ Request request_of(const TreeParams& p, int begin, in
 
 // Keys that some row of the row tile with tokens [i0, i0 + n) may see.
 __device__ __forceinline__ int keys_of(const TreeParams& p, const Request& r, int i0) {
-  int inner;
-  if (p.mask != nullptr) inner = min(r.count, 32 * p.mask_words);
-  else inner = min(r.count, i0 + p.tile_tokens);
+  const int inner = p.mask != nullptr ? min(r.count, 32 * p.mask_words) : min(r.count, i0 + p.tile_tokens);
   return min(r.ctx + inner, r.room);
 }
 
@@ -117,7 +115,11 @@ __device__ __forceinline__ long long head_tiles(const TreeParams& p, const Reque
   return n;
 }
 
-__device__ __forceinline__ long long divide(long long a, long long b) {  // a, b >= 0
+// a / b for a >= 0, b > 0. Not inlined: the scheduler divides in many places,
+// once each, and on the path from a launch to its first load code that runs
+// once costs what it takes to fetch (inlined with a fast path for small
+// numbers, it made the smallest call 3 us longer).
+__device__ __noinline__ long long divide(long long a, long long b) {
   if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
   return a / b;
 }
@@ -126,9 +128,15 @@ __device__ __forceinline__ long long divide(long long a, long long b) {  // a, b
 // floor(c total / used), so that tile u is the share of CTA
 // ceil((u + 1) used / total) - 1.
 struct Division {
-  long long total;
-  int used;
-  __device__ __forceinline__ long long begin(int c) const { return divide(c * total, used); }
+  long long total, quot;
+  int used, rem;
+  __device__ __forceinline__ void init(long long total_, int grid) {
+    total = total_;
+    used = static_cast<int>(min(static_cast<long long>(grid), total));
+    quot = used > 0 ? divide(total, used) : 0;
+    rem = static_cast<int>(total - quot * used);
+  }
+  __device__ __forceinline__ long long begin(int c) const { return c * quot + divide(c * rem, used); }
   __device__ __forceinline__ int owner(long long u) const { return static_cast<int>(divide((u + 1) * used - 1, total)); }
 };
 
@@ -172,8 +180,7 @@ struct Scheduler {
       const long long x = __shfl_up_sync(0xffffffffu, before, d);
       if (lane >= d) before += x;
     }
-    div.total = __shfl_sync(0xffffffffu, before, 31);
-    div.used = static_cast<int>(min(static_cast<long long>(p.grid), div.total));
+    div.init(__shfl_sync(0xffffffffu, before, 31), p.grid);
     before -= mine;
     s = s1 = off = 0;
     b = h = i0 = 0;
@@ -213,9 +220,24 @@ struct Scheduler {
           const long long per_head = head_tiles<kBN>(p, r);
           h = static_cast<int>(divide(off, per_head));
           off -= h * per_head;
-          while (off >= tiles_of<kBN>(p, r, i0)) {
-            off -= tiles_of<kBN>(p, r, i0);
-            i0 += p.tile_tokens;
+          if (p.mask != nullptr) {
+            const int n = tiles_of<kBN>(p, r, 0), rt = static_cast<int>(divide(off, n));
+            i0 = rt * p.tile_tokens;
+            off -= static_cast<long long>(rt) * n;
+          } else {  // 32 row tiles at a time
+            while (true) {
+              const int mine = i0 + lane * p.tile_tokens;
+              int upto = mine < r.count ? tiles_of<kBN>(p, r, mine) : 0;
+#pragma unroll
+              for (int d = 1; d < 32; d <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += x;
+              }
+              const int skip = __popc(__ballot_sync(0xffffffffu, upto <= off));
+              if (skip > 0) off -= __shfl_sync(0xffffffffu, upto, skip - 1);
+              i0 += skip * p.tile_tokens;
+              if (skip < 32) break;
+            }
           }
         }
         entered = true;
@@ -330,6 +352,18 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {
   if ((w >> 16 & e) == e) w &= 0x0000ffffu;
   return w;
 }
+// acc + 0 * w: NaN from then on if an element of w is infinite or NaN.
+__device__ __forceinline__ uint32_t taint(uint32_t acc, uint32_t w, __half) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0)),
+                            *reinterpret_cast<const __half2*>(&acc));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t taint(uint32_t acc, uint32_t w, __nv_bfloat16) {
+  const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w),
+                                   __bfloat162bfloat162(__ushort_as_bfloat16(0)),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&acc));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   uint4 v;
@@ -342,17 +376,27 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 // [mixed, valid) cleared. Returns whether any were.
 template <typename T, int HD, int kBN>
 __device__ __forceinline__ bool guard_v(uint32_t tile, int mixed, int valid, int lane) {
-  bool bad = false;
+  uint32_t acc = 0;
 #pragma unroll
   for (int hh = 0; hh < HD / 64; ++hh) {
     const uint32_t half = tile + hh * (kBN * 128);
     for (int c = valid * 8 + lane; c < kBN * 8; c += 32) st_shared_v4(half + c * 16, 0u, 0u, 0u, 0u);
+    // a first look, in which a multiplication by zero finds what is not finite
+#pragma unroll 4
     for (int c = mixed * 8 + lane; c < valid * 8; c += 32) {
       const uint4 v = ld_shared_v4(half + c * 16);
-      const uint4 f = make_uint4(finite2<T>(v.x), finite2<T>(v.y), finite2<T>(v.z), finite2<T>(v.w));
-      if (f.x != v.x || f.y != v.y || f.z != v.z || f.w != v.w) {
-        st_shared_v4(half + c * 16, f.x, f.y, f.z, f.w);
-        bad = true;
+      acc = taint(taint(taint(taint(acc, v.x, T()), v.y, T()), v.z, T()), v.w, T());
+    }
+  }
+  const bool bad = finite2<T>(acc) != acc;
+  if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll 1
+    for (int hh = 0; hh < HD / 64; ++hh) {
+      const uint32_t half = tile + hh * (kBN * 128);
+#pragma unroll 1
+      for (int c = mixed * 8 + lane; c < valid * 8; c += 32) {
+        const uint4 v = ld_shared_v4(half + c * 16);
+        st_shared_v4(half + c * 16, finite2<T>(v.x), finite2<T>(v.y), finite2<T>(v.z), finite2<T>(v.w));
       }
     }
   }
@@ -403,6 +447,16 @@ __device__ __forceinline__ void clear_padding(const TreeParams& p, int worker, i
     if (lane < HD / 8) reinterpret_cast<uint4*>(static_cast<T*>(p.out) + orow * HD)[lane] = make_uint4(0u, 0u, 0u, 0u);
     if (p.lse != nullptr && lane == 0) p.lse[orow] = -INFINITY;
   }
+}
+
+// Whether every other of the n parts has arrived, so that this CTA need not
+// put its own into memory: then the word is cleared.
+__device__ __forceinline__ bool others_arrived(unsigned long long* word, unsigned long long tag, int n) {
+  unsigned long long v;
+  asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(word) : "memory");
+  if (v != (tag << 16 | static_cast<unsigned>(n - 1))) return false;
+  *reinterpret_cast<volatile unsigned long long*>(word) = 0ull;
+  return true;
 }
 
 }  // namespace
