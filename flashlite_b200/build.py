@@ -24,7 +24,8 @@ INCLUDE = PKG.parent / "include"
 BUILD = PKG / "_build"
 
 CUDA_SOURCES = ["fl_api.cu", "fl_flash2.cu", "fl_flash2_sk.cu", "fl_flash2_bwd.cu", "fl_naive.cu",
-                "fl_noalloc.cu", "fl_selftest.cu", "fl_rotary.cu", "fl_plan.cu", "fl_tree.cu"]
+                "fl_noalloc.cu", "fl_selftest.cu", "fl_rotary.cu", "fl_plan.cu", "fl_tree.cu",
+                "fl_tree_few.cu"]
 BINDING_SOURCES = ["flash_attn.cpp", "serving.cpp"]
 HEADERS = ["fl_ptx.cuh", "fl_internal.h", "fl_flash2_common.cuh", "fl_tree_common.cuh",
            "fl_types.cuh"]

@@ -73,36 +73,6 @@ constexpr int kRegsProducer = HD == 64 ? 72 : 88;
 template <int HD>
 constexpr int kRegsSoftmax = 256 - kRegsProducer<HD>;
 
-// One step of a join, a running maximum over parts taken two (or more) at a
-// time: acc, sum and m take in parts with log2-sum-exps l and values v.
-template <int kBatch, int kVals>
-__device__ __forceinline__ void join_step(float& m, float& sum, float (&acc)[kVals], const float (&l)[kBatch],
-                                          const float (&v)[kBatch][kVals]) {
-  float m_new = m;
-#pragma unroll
-  for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, l[k]);
-  const float m_use = m_new == -INFINITY ? 0.0f : m_new, alpha = ex2_approx(m - m_use);
-  m = m_new;
-  sum *= alpha;
-#pragma unroll
-  for (int j = 0; j < kVals; ++j) acc[j] *= alpha;
-#pragma unroll
-  for (int k = 0; k < kBatch; ++k) {
-    const float w = ex2_approx(l[k] - m_use);
-    sum += w;
-#pragma unroll
-    for (int j = 0; j < kVals; ++j) acc[j] = fmaf(w, v[k][j], acc[j]);
-  }
-}
-__device__ __forceinline__ float join_inv(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
-__device__ __forceinline__ float join_lse(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
-__device__ __forceinline__ void get4(float* to, const float4& v) {
-  to[0] = v.x;
-  to[1] = v.y;
-  to[2] = v.z;
-  to[3] = v.w;
-}
-
 // Joins the n partial results base, base + stride, ... of a unit:
 //   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M),  M = max_k lse_k,
 // by the 128 softmax threads; into slot `to` or, if to < 0, out. Part i of a
@@ -249,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsProducer<HD>));
     if (warp == 3) {
       // ======================= scheduler =======================
-      Scheduler<kBN> sched(p, cta, lane);
+      Scheduler<kBN, false> sched(p, cta, lane);
       for (int ring = 0;; ++ring) {
         const Segment g = sched.next();
         const int st = ring % kSegRing;
@@ -272,7 +242,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       const int stages = is_k ? kStagesK : kStagesV;
       const CUtensorMap* tm = is_k ? &p.tm_k : &p.tm_v;
       const uint32_t ring0 = is_k ? s_k0 : s_v0, full0 = is_k ? bar_kfull : bar_vfull, empty0 = is_k ? bar_kempty : bar_vempty;
-      const int page = 1 << p.page_shift;
       int tile = 0, seg = 0, q_loads = 0;
       bool ok = true;
       while (ok) {
@@ -296,23 +265,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
           ++q_loads;
         }
         for (int t = g.t0; t < g.t1; ++t, ++tile) {
-          const int blk = pages.of_tile(g, t, is_k);
+          pages.begin_tile(t);
           const int st = tile % stages;
           if (!wait_all(empty0 + 8 * st, ((tile / stages) & 1) ^ 1, abort_flag, p.err)) {
             ok = false;
             break;
           }
-          const int live = __popc(__ballot_sync(0xffffffffu, blk >= 0));
-          if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, live * p.box_rows * 128 * C::kHalves);
-          __syncwarp();
-          if (blk >= 0) {
-            const int key = t * kBN + lane * p.box_rows;
-#pragma unroll
-            for (int hh = 0; hh < C::kHalves; ++hh)
-              tma_load_4d(ring0 + st * C::kTileBytes + hh * (kBN * 128) + lane * p.box_rows * 128, tm, full0 + 8 * st,
-                          64 * hh, key & (page - 1), g.head, blk);
-          }
-          __syncwarp();
+          load_tile<HD, kBN>(p, tm, pages, g, t, ring0 + st * C::kTileBytes, full0 + 8 * st, 0, 1, is_k);
         }
       }
       if (*abort_flag && lane == 0) {
@@ -830,9 +789,17 @@ int tree_attention(const fl_tree_attention_args* args, void* stream) {
   if (scale == 0.0) scale = 1.0 / std::sqrt(static_cast<double>(a.head_dim));
   p.scale_log2 = static_cast<float>(scale * 1.44269504088896340736);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a.dtype == FL_DTYPE_F16
-                            ? (a.head_dim == 64 ? launch<__half, 64>(p, a, s) : launch<__half, 128>(p, a, s))
-                            : (a.head_dim == 64 ? launch<__nv_bfloat16, 64>(p, a, s) : launch<__nv_bfloat16, 128>(p, a, s));
+  // Lengths lie on the device: the rows of a request, on average, choose the
+  // kernel. Any choice is right for any lengths; a request with more rows than
+  // a tile holds takes several and reads its keys for each.
+  const int64_t rows = a.requests > 0 ? (a.tokens + a.requests - 1) / a.requests * p.group : p.group;
+  cudaError_t e;
+  if (rows <= 16)
+    e = launch_tree_few(p, a, 16, s);
+  else if (a.dtype == FL_DTYPE_F16)
+    e = a.head_dim == 64 ? launch<__half, 64>(p, a, s) : launch<__half, 128>(p, a, s);
+  else
+    e = a.head_dim == 64 ? launch<__nv_bfloat16, 64>(p, a, s) : launch<__nv_bfloat16, 128>(p, a, s);
   return e == cudaSuccess ? FL_OK : cuda_fail(e, "tree attention launch");
 }
 

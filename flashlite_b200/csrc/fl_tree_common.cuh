@@ -60,7 +60,7 @@ bool encode_tree_maps(TreeParams& p, const fl_tree_attention_args& a, int tile_k
 
 namespace {
 
-constexpr int kSegRing = 4;  // work descriptors between the scheduler and the other warps
+constexpr int kSegRing = 3;  // work descriptors between the scheduler and the other warps
 
 // A reference maximum is kept until a row's maximum exceeds it by this much
 // (log2); probabilities are held 2^kUp times their size, so that fp16 keeps
@@ -143,7 +143,7 @@ struct Division {
 // A CTA's share of one unit: tiles [t0, t1) of n.
 struct Segment {
   int request, head, i0, rows;  // rows = tokens in the row tile times group
-  int begin, count, ctx, keys;
+  int begin, ctx, keys;
   int t0, t1;                   // t1 < 0: no more work
   int slot;                     // partial result, -1: the whole unit, written to out
   int part, parts;              // which of the unit's how many parts
@@ -153,18 +153,31 @@ struct Segment {
 // The scheduler of one CTA: a warp that walks over the CTA's share of the
 // tiles and hands out its segments. All lanes hold the same state, but for the
 // 32 requests from `base` on, one a lane.
-template <int kBN>
+//
+// kAligned: where a launch has fewer units than CTAs, every CTA takes at most
+// one part of one unit, all parts of a unit are of one size and short units
+// stay whole. Joining costs some 4 us on the way to the result, as much as
+// kWholeTiles tiles; and parts at like places of neighbouring key heads run
+// side by side, which read the same rows of memory where heads are
+// interleaved.
+constexpr int kWholeTiles = 8;
+
+template <int kBN, bool kAligned>
 struct Scheduler {
   const TreeParams& p;
   const int cta, lane;
   Division div;
+  int part_tiles;        // aligned: tiles of a part; 0: even division
   long long s, s1, off;  // next tile, end of the share, tiles of the current request before s
   int b, h, i0;          // request, key head, first token of the row tile
   bool entered;          // whether h and i0 are those of request b
   int base, l_begin, l_end, l_ctx;
   Request r;
 
-  __device__ __forceinline__ Scheduler(const TreeParams& p_, int cta_, int lane_) : p(p_), cta(cta_), lane(lane_) {
+  // used = false: a warp that only has the object.
+  __device__ __forceinline__ Scheduler(const TreeParams& p_, int cta_, int lane_, bool used = true)
+      : p(p_), cta(cta_), lane(lane_) {
+    if (!used) return;
     load(0);
     const int per = (p.requests + 31) / 32;  // each lane sums a run of requests
     const int b0 = min(lane * per, p.requests), b1 = min(b0 + per, p.requests);
@@ -185,6 +198,22 @@ struct Scheduler {
     s = s1 = off = 0;
     b = h = i0 = 0;
     entered = false;
+    part_tiles = 0;
+    if constexpr (kAligned) {
+      if (p.requests <= 32) {
+        const Request r = request_of(p, l_begin, l_end, l_ctx, false);
+        const int row_tiles = lane < p.requests ? (r.count + p.tile_tokens - 1) / p.tile_tokens : 0;
+        const long long units = __reduce_add_sync(0xffffffffu, row_tiles) * static_cast<long long>(p.kv_heads);
+        if (units < p.grid) {
+          const long long m = divide(div.total + p.grid - units - 1, p.grid - units);  // sum of ceil(n / m) <= grid
+          if (m <= kWholeTiles || 8 * m * p.grid <= 9 * div.total) part_tiles = static_cast<int>(max(m, 2LL));
+        }
+        if (part_tiles > 0) {
+          aligned(r, row_tiles);
+          return;
+        }
+      }
+    }
     if (cta >= div.used) return;
     s = div.begin(cta);
     s1 = div.begin(cta + 1);
@@ -204,11 +233,52 @@ struct Scheduler {
     off = __shfl_sync(0xffffffffu, off, owner);
   }
 
+  __device__ __forceinline__ int parts_of(int n) const {
+    return n <= max(part_tiles, kWholeTiles) ? 1 : static_cast<int>(divide(n + part_tiles - 1, part_tiles));
+  }
+  // Finds part number `cta` of all: request b (lane b), key head h, first token
+  // i0 and, as s, the part's number within the unit. s1 = s: there is none.
+  __device__ __forceinline__ void aligned(const Request& r, int row_tiles) {
+    int per_head = 0;
+    for (int i = 0; i < row_tiles; ++i) per_head += parts_of(tiles_of<kBN>(p, r, i * p.tile_tokens));
+    const int mine = per_head * p.kv_heads;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    const uint32_t after = __ballot_sync(0xffffffffu, upto > cta);
+    if (after == 0) return;
+    b = __ffs(after) - 1;
+    int rest = cta - __shfl_sync(0xffffffffu, upto - mine, b);
+    const int ph = __shfl_sync(0xffffffffu, per_head, b);
+    h = static_cast<int>(divide(rest, ph));
+    rest -= h * ph;
+    this->r = request_of(p, __shfl_sync(0xffffffffu, l_begin, b), __shfl_sync(0xffffffffu, l_end, b),
+                         __shfl_sync(0xffffffffu, l_ctx, b), false);
+    for (int n; rest >= (n = parts_of(tiles_of<kBN>(p, this->r, i0))); i0 += p.tile_tokens) rest -= n;
+    s = rest;
+    s1 = rest + 1;
+  }
+
   // The next segment, or t1 = -1 after the last.
   __device__ __forceinline__ Segment next() {
     Segment g = {};
     g.t1 = -1;
     if (s >= s1) return g;
+    if (kAligned && part_tiles > 0) {
+      const int n = tiles_of<kBN>(p, r, i0);
+      fill(g);
+      g.parts = parts_of(n);
+      g.part = static_cast<int>(s);
+      // parts of one size, or one tile less
+      g.t0 = static_cast<int>(divide(static_cast<long long>(g.part) * n, g.parts));
+      g.t1 = static_cast<int>(divide(static_cast<long long>(g.part + 1) * n, g.parts));
+      g.slot = g.parts == 1 ? -1 : 2 * cta + (g.part == 0 ? 1 : 0);
+      s1 = s;
+      return g;
+    }
     while (true) {
       if (!entered) {
         if (b >= p.requests) return g;
@@ -252,14 +322,7 @@ struct Scheduler {
       entered = false;
     }
     const int n = tiles_of<kBN>(p, r, i0);
-    g.request = b;
-    g.head = h;
-    g.i0 = i0;
-    g.rows = min(p.tile_tokens, r.count - i0) * p.group;
-    g.begin = r.begin;
-    g.count = r.count;
-    g.ctx = r.ctx;
-    g.keys = keys_of(p, r, i0);
+    fill(g);
     g.t0 = static_cast<int>(off);
     g.t1 = static_cast<int>(min(static_cast<long long>(n), off + (s1 - s)));
     const bool whole = g.t0 == 0 && g.t1 == n;
@@ -278,6 +341,15 @@ struct Scheduler {
   }
 
  private:
+  __device__ __forceinline__ void fill(Segment& g) const {
+    g.request = b;
+    g.head = h;
+    g.i0 = i0;
+    g.rows = min(p.tile_tokens, r.count - i0) * p.group;
+    g.begin = r.begin;
+    g.ctx = r.ctx;
+    g.keys = keys_of(p, r, i0);
+  }
   __device__ __forceinline__ void load(int from) {
     base = from;
     const int x = from + lane;
@@ -295,8 +367,7 @@ struct Scheduler {
 
 // Block numbers of a segment's pages, for a producer warp: 32 at a time, one a
 // lane, and the next 32 already under way. (Read one tile ahead, they arrived
-// too late once the memory was busy: 3,000 cycles a tile where the tile itself
-// needed 1,500.)
+// too late once the memory was busy.)
 template <int kBN>
 struct PageNumbers {
   const TreeParams& p;
@@ -310,25 +381,54 @@ struct PageNumbers {
     cur = load(base + lane);
     next = load(base + 32 + lane);
   }
-  // The block of this lane's box of tile t; -1: no box, num_blocks (outside
-  // the map: zeros arrive and nothing is read) for a number out of range.
-  __device__ __forceinline__ int of_tile(const Segment& g, int t, bool report) {
+  __device__ __forceinline__ void begin_tile(int t) {
     if ((t * kBN >> p.page_shift) - base >= 32) {
       cur = next;
       base += 32;
       next = load(base + 32 + lane);
     }
-    const int key = t * kBN + lane * p.box_rows;
+  }
+  // Page boxes of tile t that hold visible keys.
+  __device__ __forceinline__ int boxes(const Segment& g, int t) const {
+    return (max(0, min(kBN, g.keys - t * kBN)) + p.box_rows - 1) / p.box_rows;
+  }
+  // The block with this lane's key; num_blocks (outside the map: zeros arrive
+  // and nothing is read) for a number out of range.
+  __device__ __forceinline__ int block(int key, bool live, bool report) const {
     const int blk = __shfl_sync(0xffffffffu, cur, (key >> p.page_shift) - base);
-    if (lane >= kBN / p.box_rows || key >= g.keys) return -1;
     if (blk >= 0 && blk < p.num_blocks) return blk;
-    if (report) atomicOr(p.err, kDevErrIndex);
+    if (live && report) atomicOr(p.err, kDevErrIndex);
     return p.num_blocks;
   }
 
  private:
   __device__ __forceinline__ int load(int page) const { return page <= last ? row[page] : 0; }
 };
+
+// Warp `worker` of `workers` loads its share of tile t's page boxes into
+// shared memory ([kBN][64-column halves]), completing on `bar`; a lane for
+// each box. A copy takes its warp some 125 cycles to issue, however it is
+// written, so that small pages want several warps.
+template <int HD, int kBN>
+__device__ __forceinline__ void load_tile(const TreeParams& p, const CUtensorMap* tm, const PageNumbers<kBN>& pages,
+                                          const Segment& g, int t, uint32_t dst, uint32_t bar, int worker, int workers,
+                                          bool report) {
+  const int lane = pages.lane, n = pages.boxes(g, t);
+  if (worker == 0) {
+    if (lane == 0) mbar_arrive_expect_tx(bar, n * p.box_rows * 128 * (HD / 64));
+    __syncwarp();
+  }
+  const int box = lane * workers + worker, key = t * kBN + box * p.box_rows;
+  const bool live = box < n;
+  const int blk = pages.block(key, live, report);
+  if (live) {
+#pragma unroll
+    for (int hh = 0; hh < HD / 64; ++hh)
+      tma_load_4d(dst + hh * (kBN * 128) + box * p.box_rows * 128, tm, bar, 64 * hh, key & ((1 << p.page_shift) - 1), g.head,
+                  blk);
+  }
+  __syncwarp();
+}
 
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err));
@@ -434,6 +534,36 @@ __device__ __forceinline__ bool arrive_last(unsigned long long* word, int n) {
   if (static_cast<int>(old & 0xffffu) + 1 != n) return false;
   *reinterpret_cast<volatile unsigned long long*>(word) = 0ull;
   return true;
+}
+
+// One step of a join, a running maximum over parts taken two (or more) at a
+// time: acc, sum and m take in parts with log2-sum-exps l and values v.
+template <int kBatch, int kVals>
+__device__ __forceinline__ void join_step(float& m, float& sum, float (&acc)[kVals], const float (&l)[kBatch],
+                                          const float (&v)[kBatch][kVals]) {
+  float m_new = m;
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, l[k]);
+  const float m_use = m_new == -INFINITY ? 0.0f : m_new, alpha = ex2_approx(m - m_use);
+  m = m_new;
+  sum *= alpha;
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) acc[j] *= alpha;
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k) {
+    const float w = ex2_approx(l[k] - m_use);
+    sum += w;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) acc[j] = fmaf(w, v[k][j], acc[j]);
+  }
+}
+__device__ __forceinline__ float join_inv(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+__device__ __forceinline__ float join_lse(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
+__device__ __forceinline__ void get4(float* to, const float4& v) {
+  to[0] = v.x;
+  to[1] = v.y;
+  to[2] = v.z;
+  to[3] = v.w;
 }
 
 // Rows of q that belong to no request (a batch padded to a fixed size): by

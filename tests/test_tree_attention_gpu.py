@@ -210,6 +210,18 @@ def test_many_short_requests(cuda):
     Case(cuda, [(rng.randint(0, 40), rng.randint(0, 2)) for _ in range(700)], 4, 2, 64, 16).check()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,tokens", [(8, 1), (4, 6), (8, 9)])
+def test_ragged_batches(cuda, dim, dtype, heads, tokens):
+    """More units than CTAs, each with its share of several: the pipeline runs on from unit to unit, through caches of
+    no tile to a dozen, whatever the parity of what it has done before."""
+    rng = random.Random(heads * tokens)
+    lengths = [(rng.choice([0, 5, 128, 300, 700, 1500]), rng.randint(0, tokens)) for _ in range(90)]
+    Case(cuda, lengths, heads, 8 if heads == 8 else 4, dim, 16, dtype, words=1 if tokens > 1 else 0, seed=tokens,
+         poison=True).check()
+
+
 def test_repeatable(cuda):
     """The same bits every time: no sum depends on the order in which parts finish."""
     c = Case(cuda, [(9000, 4), (501, 4), (33, 4)], 8, 2, 128, 16)
