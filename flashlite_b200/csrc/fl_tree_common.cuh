@@ -156,11 +156,13 @@ struct Segment {
 //
 // kAligned: where a launch has fewer units than CTAs, every CTA takes at most
 // one part of one unit, all parts of a unit are of one size and short units
-// stay whole. Joining costs some 4 us on the way to the result, as much as
-// kWholeTiles tiles; and parts at like places of neighbouring key heads run
-// side by side, which read the same rows of memory where heads are
-// interleaved.
-constexpr int kWholeTiles = 8;
+// stay whole: joining costs 3 us on the way to the result, as much as
+// kWholeTiles tiles. Parts at like places of neighbouring key heads run side
+// by side, which read the same rows of memory where heads are interleaved. The
+// division is taken where it is within an eighth of even (one cache of 131072
+// keys, 8 heads: 57 us for 63) or its parts are short all the same (8 requests
+// of up to 4096 keys: 17.6 us for 22.1, few cuts against many).
+constexpr int kWholeTiles = 3, kShortPart = 8;
 
 template <int kBN, bool kAligned>
 struct Scheduler {
@@ -206,7 +208,7 @@ struct Scheduler {
         const long long units = __reduce_add_sync(0xffffffffu, row_tiles) * static_cast<long long>(p.kv_heads);
         if (units < p.grid) {
           const long long m = divide(div.total + p.grid - units - 1, p.grid - units);  // sum of ceil(n / m) <= grid
-          if (m <= kWholeTiles || 8 * m * p.grid <= 9 * div.total) part_tiles = static_cast<int>(max(m, 2LL));
+          if (m <= kShortPart || 8 * m * p.grid <= 9 * div.total) part_tiles = static_cast<int>(max(m, 1LL));
         }
         if (part_tiles > 0) {
           aligned(r, row_tiles);
