@@ -52,9 +52,10 @@ struct TreeParams {
   int grid;
 };
 
-// Attention of few rows (fl_tree_few.cu): rows 16 or 32 to a unit. The caller
+// Attention of few rows (fl_tree_few.cu): up to kFewRows to a unit. The caller
 // has filled in everything but what depends on the kernel's tiles.
-cudaError_t launch_tree_few(TreeParams& p, const fl_tree_attention_args& a, int rows, cudaStream_t stream);
+constexpr int kFewRows = 16;
+cudaError_t launch_tree_few(TreeParams& p, const fl_tree_attention_args& a, cudaStream_t stream);
 // Tensor maps of q, the caches for tiles of kBN keys and row tiles of p.tile_tokens.
 bool encode_tree_maps(TreeParams& p, const fl_tree_attention_args& a, int tile_keys);
 

@@ -1,27 +1,28 @@
-// Attention over a paged cache for few rows: up to 16 or 32 to a unit, the
-// tokens of a request times the query heads that share a key head (decoding
-// single tokens, small trees). Same mathematics as fl_tree.cu.
+// Attention over a paged cache for few rows: up to 16 to a unit, the tokens of
+// a request times the query heads that share a key head (decoding single
+// tokens, small trees). Same mathematics as fl_tree.cu.
 //
-// Bound by the keys and values read once from memory; what has to be kept out
-// of their way is latency. With S = Q K^T as a 128-row product, 4 to 32 rows
-// would leave one softmax warp of four with work, on one quarter of the SM.
-// So the products are transposed:
-//   S^T = K Q^T      A = K tile (128 keys), B = Q (16 or 32 rows)
+// Bound by the keys and values read once from memory, and for small calls by
+// latency. With S = Q K^T as a 128-row product, so few rows would leave one
+// softmax warp of four with work, on one quarter of the SM. So the products
+// are transposed:
+//   S^T = K Q^T      A = K tile (128 keys), B = Q (16 rows)
 //   O^T += V^T P^T   A = V tile, read MN-major, B = P^T
-// A TMEM lane, and a softmax thread, is a key with all the rows' scores: the
-// exponentials spread over all four warps, and 128 keys x 16 rows cost a warp
-// some 250 instructions (1,200 cycles a 64-key tile before). The row maximum
-// would be a reduction across the CTA; instead every thread compares its
-// scores with the rows' common reference, and only when one exceeds it by
-// more than the lag (once a unit as a rule; one barrier with an OR tells) the
-// maxima are formed. The row sums stay in each thread until the end. O^T has
-// the head dimension along the lanes, so that a warp writes a row's
-// neighbouring columns.
+// A TMEM lane, and a softmax thread, is a key with all the rows' scores: a
+// tile's softmax takes 550 cycles for 128 keys, 1,300 for 64 the other way.
+// The row maximum would be a reduction across the CTA; instead every thread
+// compares its scores with the rows' common reference, and only when one
+// exceeds it by more than the lag (once a unit as a rule; one barrier with an
+// OR tells) the maxima are formed. The row sums stay in each thread until the
+// end. O^T has the head dimension along the lanes, so that a warp writes a
+// row's neighbouring columns.
 //
-// One CTA per SM: a scheduler warp, a producer warp that streams Q, K and V
-// through one ring (192 KB under way), an MMA warp and the softmax warpgroup.
-// S, P and O are double-buffered; the MMA warp issues whichever product is
-// ready, so that it never holds a V tile while it waits for the next K tile.
+// Two CTAs per SM, as one alone left the SMs uneven (one cache of 131072 keys:
+// 88 us for 57): two producer warps, of which one is the scheduler too, that
+// stream Q, K and V through one ring of 96 KB, an MMA warp for each product,
+// the softmax warpgroup. S, P and O are double-buffered. Measured: 64 requests
+// of up to 8192 keys, 32 heads over 8 of 128, bf16: 197 us, 6.3 TB/s, 96 % of
+// the measured copy rate; one request of 777 keys, 8 heads of 64: 11.5 us.
 
 #include <algorithm>
 #include <cmath>
@@ -34,20 +35,21 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBN = 128;  // keys per tile (UMMA M)
+constexpr int kRows = kFewRows;  // rows per unit (UMMA N): a P^T row is 32 bytes, one 32-byte swizzle atom
+static_assert(kRows == 16, "one 32-byte swizzle atom");
 constexpr int kCtasPerSm = 2;
 constexpr int kProducers = 2;  // warps 0 and 3
 // Register split: 128 x 112 (producers, MMA) + 128 x 144 (softmax) = 256 x 128, the launch's total.
 constexpr int kRegsProducer = 112, kRegsSoftmax = 144;
 
-template <int HD, int NR>
+template <int HD>
 struct Few {
   static_assert(HD == 64 || HD == 128, "head dimension 64 or 128");
-  static_assert(NR == 16 || NR == 32, "16 or 32 rows (one swizzle atom of P^T)");
   static constexpr int kHalves = HD / 64;
   static constexpr int kTileBytes = kBN * HD * 2;        // 16 / 32 KB
   static constexpr int kStages = 96 * 1024 / kTileBytes;  // K and V tiles in turn
-  static constexpr int kQBytes = NR * HD * 2;
-  static constexpr int kPBytes = kBN * NR * 2;
+  static constexpr int kQBytes = kRows * HD * 2;
+  static constexpr int kPBytes = kBN * kRows * 2;
   static constexpr int kSmemQ = kStages * kTileBytes;      // 2 buffers
   static constexpr int kSmemP = kSmemQ + 2 * kQBytes;      // 2 buffers
   static constexpr int kSmemMisc = kSmemP + 2 * kPBytes;
@@ -59,40 +61,28 @@ struct Few {
   static constexpr int kFull = kStages % 2 == 0 ? kStages : 2 * kStages;
   static __device__ __forceinline__ uint32_t full(uint32_t bar_full, int n) { return bar_full + 8 * (n % kFull); }
   static __device__ __forceinline__ uint32_t full_phase(int n) { return (n / kFull) & 1; }
-  // barriers | segments | maxima [4][NR] or sums [4][NR][2] | 1 / sum [NR] | flags
+  // barriers | segments | maxima [4][kRows] or sums [4][kRows][2] | 1 / sum [kRows] | flags
   static constexpr int kBars = kFull + kStages + 2 * kSegRing + 2 * 9 + 1;
   static constexpr int kOffSeg = (kBars * 8 + 15) / 16 * 16;
   static constexpr int kOffMax = kOffSeg + kSegRing * static_cast<int>(sizeof(Segment));
   static constexpr int kOffSum = kOffMax;  // never in use at the same time: a barrier lies between
-  static constexpr int kOffInv = kOffMax + 8 * NR * 4;
-  static constexpr int kOffFlag = kOffInv + NR * 4;
+  static constexpr int kOffInv = kOffMax + 8 * kRows * 4;
+  static constexpr int kOffFlag = kOffInv + kRows * 4;
   static constexpr int kSmemBytes = kSmemMisc + kOffFlag + 20;
   static_assert(kOffMax % 16 == 0, "maxima are read four at a time");
   static_assert(kCtasPerSm * (kSmemBytes + 1024) <= 228 * 1024, "shared memory");
-  static constexpr uint32_t kTmemCols = 4 * NR;            // S, O: two buffers of NR columns each
+  static constexpr uint32_t kTmemCols = 4 * kRows;            // S, O: two buffers of kRows columns each
 };
 
-// P^T rows (NR elements of a key) are 32 or 64 bytes: one swizzle atom wide.
-template <int NR>
 __device__ __forceinline__ uint64_t make_sdesc_p(uint32_t saddr) {
-  constexpr uint64_t layout = NR == 16 ? 6 : 4;  // 32- or 64-byte swizzle
-  uint64_t d = make_sdesc_sw128(saddr, 16, NR * 2 * 8);
-  return (d & ~(7ull << 61)) | layout << 61;
+  constexpr uint64_t kLayout32 = 6;  // 32-byte swizzle
+  const uint64_t d = make_sdesc_sw128(saddr, 16, kRows * 2 * 8);
+  return (d & ~(7ull << 61)) | kLayout32 << 61;
 }
 
-template <int NR>
-__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&r)[NR]) {
-  if constexpr (NR == 32) {
-    tmem_ld32_wait(addr, r);
-  } else {
-    tmem_ld16_nowait(addr, r);
-    tmem_wait_ld16_dep(r);
-  }
-}
-template <int NR>
-__device__ __forceinline__ void tmem_st_rows(uint32_t addr, const uint32_t (&r)[NR]) {
-  if constexpr (NR == 32) tmem_st32(addr, r);
-  else tmem_st16(addr, r);
+__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&r)[kRows]) {
+  tmem_ld16_nowait(addr, r);
+  tmem_wait_ld16_dep(r);
 }
 
 // Barrier of the 128 softmax threads that also tells whether any had `x`.
@@ -117,44 +107,23 @@ __device__ __forceinline__ float warp_max(float x) {
   return y;
 }
 
-// Sums over a warp of NR values per lane: lane l ends with that of row
-// row_of_lane(l). Halves the values each time, so NR shuffles and not 5 NR.
-template <int NR>
-__device__ __forceinline__ float warp_sums(float (&a)[NR], int lane) {
-  int half = NR / 2;
+// Sums over a warp of kRows values per lane: lanes 2 r and 2 r + 1 end with
+// that of row r. Each step halves the values: 16 shuffles, not 80.
+__device__ __forceinline__ float warp_sums(float (&a)[kRows], int lane) {
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    if (half > 0) {
+  for (int half = kRows / 2, d = 16; half > 0; half /= 2, d /= 2) {
+    const bool up = lane & d;
 #pragma unroll
-      for (int i = 0; i < NR / 2; ++i) {
-        if (i < half) {
-          const bool up = lane & d;
-          const float send = up ? a[i] : a[i + half], keep = up ? a[i + half] : a[i];
-          a[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
-        }
-      }
-      half /= 2;
-    } else {
-      a[0] += __shfl_xor_sync(0xffffffffu, a[0], d);
+    for (int i = 0; i < half; ++i) {
+      const float send = up ? a[i] : a[i + half], keep = up ? a[i + half] : a[i];
+      a[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
     }
   }
-  return a[0];
+  return a[0] + __shfl_xor_sync(0xffffffffu, a[0], 1);
 }
-template <int NR>
-__device__ __forceinline__ int row_of_lane(int lane) {
-  int row = 0, half = NR / 2;
-#pragma unroll
-  for (int d = 16; d; d >>= 1)
-    if (half > 0) {
-      row += (lane & d) ? half : 0;
-      half /= 2;
-    }
-  return row;
-}
-
-template <typename T, int HD, int NR>
+template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __grid_constant__ TreeParams p) {
-  using C = Few<HD, NR>;
+  using C = Few<HD>;
   constexpr int kStages = C::kStages;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -251,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           mbar_arrive_expect_tx(bar_qfull + 8 * (seg & 1), p.group * p.tile_tokens * 128 * C::kHalves);
 #pragma unroll
           for (int hh = 0; hh < C::kHalves; ++hh)
-            tma_load_3d(s_q + (seg & 1) * C::kQBytes + hh * (NR * 128), &p.tm_q, bar_qfull + 8 * (seg & 1), 64 * hh,
+            tma_load_3d(s_q + (seg & 1) * C::kQBytes + hh * (kRows * 128), &p.tm_q, bar_qfull + 8 * (seg & 1), 64 * hh,
                         g.head * p.group, g.begin + g.i0);
         }
         __syncwarp();
@@ -283,10 +252,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
     }
   } else if (warp == 1) {
     // ======================= S^T = K Q^T =======================
-    constexpr uint32_t idesc = make_idesc_f16_f32(kBN, NR, false, false, kBf16);  // K-major A (K) and B (Q)
+    constexpr uint32_t idesc = make_idesc_f16_f32(kBN, kRows, false, false, kBf16);  // K-major A (K) and B (Q)
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint64_t dk0 = make_sdesc_sw128(sbase, 16, 1024), dq0 = make_sdesc_sw128(s_q, 16, 1024);
-    constexpr uint64_t kTileEnc = C::kTileBytes >> 4, kKHalf = (kBN * 128) >> 4, kQHalf = (NR * 128) >> 4;
+    constexpr uint64_t kTileEnc = C::kTileBytes >> 4, kKHalf = (kBN * 128) >> 4, kQHalf = (kRows * 128) >> 4;
     int js = 0, seg = 0;
     bool ok = true;
     while (ok) {
@@ -307,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
-            umma_f16_ss(tm + (js & 1) * NR, ad + 2 * (kk & 3) + (kk >> 2) * kKHalf, bd + 2 * (kk & 3) + (kk >> 2) * kQHalf,
+            umma_f16_ss(tm + (js & 1) * kRows, ad + 2 * (kk & 3) + (kk >> 2) * kKHalf, bd + 2 * (kk & 3) + (kk >> 2) * kQHalf,
                         idesc, kk > 0 ? 1u : 0u);
           umma_commit(bar_s + 8 * (js & 1));
           umma_commit(bar_empty + 8 * st);
@@ -327,11 +296,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
     // ======================= O^T += V^T P^T (warp 2) =======================
     // A warp of its own: it never holds a V tile while it waits for the next K
     // tile, and either product goes out as soon as it can.
-    constexpr uint32_t idesc = make_idesc_f16_f32(kBN, NR, true, true, kBf16);  // MN-major A (V) and B (P)
+    constexpr uint32_t idesc = make_idesc_f16_f32(kBN, kRows, true, true, kBf16);  // MN-major A (V) and B (P)
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     // 64-column halves of V one leading offset apart. With head dimension 64
     // the product's rows 64-127 are whatever lies there: not looked at.
-    const uint64_t dv0 = make_sdesc_sw128(sbase, HD == 64 ? 8192 : kBN * 128, 1024), dp0 = make_sdesc_p<NR>(s_p);
+    const uint64_t dv0 = make_sdesc_sw128(sbase, HD == 64 ? 8192 : kBN * 128, 1024), dp0 = make_sdesc_p(s_p);
     constexpr uint64_t kTileEnc = C::kTileBytes >> 4;
     int js = 0, seg = 0;
     bool ok = true;
@@ -363,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kBN / 16; ++kk)
-            umma_f16_ss(tm + 2 * NR + o * NR, ad + 128 * kk, bd + kk * (NR * 2 * 16 >> 4), idesc, kk > 0 ? 1u : accumulate);
+            umma_f16_ss(tm + 2 * kRows + o * kRows, ad + 128 * kk, bd + kk * (kRows * 2 * 16 >> 4), idesc, kk > 0 ? 1u : accumulate);
           umma_commit(bar_pv + 8 * (js & 1));
           umma_commit(bar_empty + 8 * st);
         }
@@ -386,9 +355,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
     const int t_key = tid - 128;  // also the column of O this thread holds
     const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const float sc = p.scale_log2;
-    // this thread's key in a P buffer: NR elements, 16-byte chunks swizzled as the product reads them
-    const uint32_t p_row = s_p + t_key * (NR * 2);
-    const int swz = NR == 16 ? (t_key >> 2) & 1 : (t_key >> 1) & 3;
+    // this thread's key in a P buffer: kRows elements, 16-byte chunks swizzled as the product reads them
+    const uint32_t p_row = s_p + t_key * (kRows * 2);
+    const int swz = (t_key >> 2) & 1;
     constexpr float kNone = -3.0e38f;  // reference of a row that has seen nothing
     int js = 0, seg = 0;               // tiles and segments so far
     // A wait that gives up clears ok. The four warps meet at barriers, so none
@@ -403,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
       if (lane == 0) mbar_arrive(bar_segempty + 8 * sl);
       if (g.t1 < 0) break;
       const uint32_t all_rows = g.rows >= 32 ? 0xffffffffu : (1u << g.rows) - 1u;
-      const uint32_t tO = tmem + lane_base + 2 * NR + (seg & 1) * NR;
+      const uint32_t tO = tmem + lane_base + 2 * kRows + (seg & 1) * kRows;
       // rows of the tile that see new token j of the request
       auto rows_seeing = [&](int j) -> uint32_t {
         if (p.mask == nullptr) {
@@ -417,9 +386,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
               seen |= (p.group >= 32 ? 0xffffffffu : (1u << p.group) - 1u) << r;
         return seen & all_rows;
       };
-      float ref[NR], l[NR], lr[NR];  // reference maxima less kUp; sums of p, and of p as rounded for the product
+      float ref[kRows], l[kRows], lr[kRows];  // reference maxima less kUp; sums of p, and of p as rounded for the product
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
+      for (int r = 0; r < kRows; ++r) {
         ref[r] = kNone;
         l[r] = lr[r] = 0.0f;
       }
@@ -429,16 +398,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
         const uint32_t vis = key < g.ctx ? (key < g.keys ? all_rows : 0u) : key < g.keys ? rows_seeing(key - g.ctx) : 0u;
         ok = ok && wait_all(bar_s + 8 * buf, (js >> 1) & 1, abort_flag, p.err);
         tc_fence_after();
-        uint32_t sr[NR];
-        tmem_ld_rows<NR>(tmem + lane_base + buf * NR, sr);
+        uint32_t sr[kRows];
+        tmem_ld_rows(tmem + lane_base + buf * kRows, sr);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_sfree + 8 * buf);
         // Scaled first: a fused multiply-add against a rounded reference could
         // be off by more than the lag where scores are large.
-        float y[NR], most = -INFINITY;
+        float y[kRows], most = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
+        for (int r = 0; r < kRows; ++r) {
           y[r] = (vis >> r & 1u) ? __uint_as_float(sr[r]) * sc : -INFINITY;
           most = fmaxf(most, y[r] - ref[r]);
         }
@@ -449,14 +418,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           }
           // new maxima: over the warp, then the four warps
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
+          for (int r = 0; r < kRows; ++r) {
             const float m = warp_max(y[r]);
             if (lane == 0) s_max[4 * r + (warp & 3)] = m;
           }
           softmax_sync();
-          float alpha[NR];
+          float alpha[kRows];
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
+          for (int r = 0; r < kRows; ++r) {
             const float4 w = reinterpret_cast<const float4*>(s_max)[r];
             const float m = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
             const float next = m - ref[r] > kLag + kUp ? m - kUp : ref[r];
@@ -468,18 +437,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           if (t > g.t0) {  // O takes the new reference when the last P V is in it
             ok = wait_all(bar_pv + 8 * (buf ^ 1), ((js - 1) >> 1) & 1, abort_flag, p.err);
             tc_fence_after();
-            uint32_t o[NR];
-            tmem_ld_rows<NR>(tO, o);
+            uint32_t o[kRows];
+            tmem_ld_rows(tO, o);
 #pragma unroll
-            for (int r = 0; r < NR; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * alpha[r]);
-            tmem_st_rows<NR>(tO, o);
+            for (int r = 0; r < kRows; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * alpha[r]);
+            tmem_st16(tO, o);
             tmem_st_wait();
             tc_fence_before();
           }
         }
-        uint32_t pk[NR / 2];
+        uint32_t pk[kRows / 2];
 #pragma unroll
-        for (int r = 0; r < NR; r += 2) {
+        for (int r = 0; r < kRows; r += 2) {
           const float a = ex2_approx(y[r] - ref[r]), b = ex2_approx(y[r + 1] - ref[r + 1]);
           l[r] += a;
           l[r + 1] += b;
@@ -491,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
         // the P V that read this buffer two tiles ago is done
         if (js >= 2) ok = ok && wait_all(bar_pv + 8 * buf, ((js >> 1) & 1) ^ 1, abort_flag, p.err);
 #pragma unroll
-        for (int c = 0; c < NR / 8; ++c)
+        for (int c = 0; c < kRows / 8; ++c)
           st_shared_v4(p_row + buf * C::kPBytes + ((c ^ swz) << 4), pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
         fence_proxy_async_smem();
         __syncwarp();
@@ -501,11 +470,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
 
       // ---- epilogue of the segment: row sums, then O ----
       {
-        const float sum = warp_sums<NR>(l, lane), sum_r = warp_sums<NR>(lr, lane);
-        const int r = row_of_lane<NR>(lane);
-        if (NR == 32 || (lane & 1) == 0) {
-          s_sum[((warp & 3) * NR + r) * 2] = sum;
-          s_sum[((warp & 3) * NR + r) * 2 + 1] = sum_r;
+        const float sum = warp_sums(l, lane), sum_r = warp_sums(lr, lane);
+        const int r = lane >> 1;
+        if ((lane & 1) == 0) {
+          s_sum[((warp & 3) * kRows + r) * 2] = sum;
+          s_sum[((warp & 3) * kRows + r) * 2 + 1] = sum_r;
         }
       }
       softmax_sync();
@@ -513,15 +482,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
         float sum = 0.0f, sum_r = 0.0f, m = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          sum += s_sum[(w * NR + t_key) * 2];
-          sum_r += s_sum[(w * NR + t_key) * 2 + 1];
+          sum += s_sum[(w * kRows + t_key) * 2];
+          sum_r += s_sum[(w * kRows + t_key) * 2 + 1];
         }
 #pragma unroll
-        for (int r = 0; r < NR; ++r) m = r == t_key ? ref[r] : m;
+        for (int r = 0; r < kRows; ++r) m = r == t_key ? ref[r] : m;
         s_inv[t_key] = sum == 0.0f ? 0.0f : 1.0f / sum_r;
         const float lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
         if (g.slot >= 0)
-          p.part_lse[g.slot * NR + t_key] = lse2;
+          p.part_lse[g.slot * kRows + t_key] = lse2;
         else if (p.lse != nullptr)
           p.lse[static_cast<long long>(g.begin + g.i0 + t_key / p.group) * p.heads + g.head * p.group + t_key % p.group] =
               lse2 * 0.69314718055994531f;
@@ -532,11 +501,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
       tc_fence_after();
       const bool bad = bad_flag[seg & 1] != 0;
       if (32 * (warp & 3) < HD) {
-        uint32_t sr[NR];
-        tmem_ld_rows<NR>(tO, sr);
-        float o[NR];
+        uint32_t sr[kRows];
+        tmem_ld_rows(tO, sr);
+        float o[kRows];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) o[r] = r < g.rows ? __uint_as_float(sr[r]) * s_inv[r] : 0.0f;
+        for (int r = 0; r < kRows; ++r) o[r] = r < g.rows ? __uint_as_float(sr[r]) * s_inv[r] : 0.0f;
         if (bad) {
           // infinities and NaN that guard_v cleared, for the rows that see them
           const int hidden = p.mask != nullptr ? g.ctx : g.ctx + g.i0 + 1;
@@ -548,14 +517,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
             if (fabsf(x) < INFINITY) continue;
             const uint32_t seen = rows_seeing(key - g.ctx);
 #pragma unroll
-            for (int r = 0; r < NR; ++r)
+            for (int r = 0; r < kRows; ++r)
               if (seen >> r & 1u) o[r] += x;
           }
         }
         if (g.slot >= 0) {
-          float* to = p.part + static_cast<long long>(g.slot) * NR * HD + t_key;
+          float* to = p.part + static_cast<long long>(g.slot) * kRows * HD + t_key;
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
+          for (int r = 0; r < kRows; ++r)
             if (r < g.rows) to[r * HD] = o[r];
         } else {
           T* to = static_cast<T*>(p.out) +
@@ -563,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           const long long next_token = static_cast<long long>(p.heads - p.group) * HD;
           int left = p.group;
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
+          for (int r = 0; r < kRows; ++r) {
             if (r >= g.rows) break;
             *to = static_cast<T>(o[r]);
             to += HD;
@@ -607,8 +576,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
               for (int k = 0; k < kBatch; ++k) {
                 const bool in = k0 + k < n;
                 const int sl = slot_of(first, base + min(k0 + k, n - 1) * stride);
-                l2[k] = in ? __ldcg(p.part_lse + sl * NR + r) : -INFINITY;
-                get4(v[k], in ? __ldcg(reinterpret_cast<const float4*>(p.part + (static_cast<long long>(sl) * NR + r) * HD) + c)
+                l2[k] = in ? __ldcg(p.part_lse + sl * kRows + r) : -INFINITY;
+                get4(v[k], in ? __ldcg(reinterpret_cast<const float4*>(p.part + (static_cast<long long>(sl) * kRows + r) * HD) + c)
                               : make_float4(0.f, 0.f, 0.f, 0.f));
               }
               join_step<kBatch, 4>(m, sum, acc, l2, v);
@@ -617,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
             const float4 o = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
             lse2 = join_lse(m, sum);
             if (to >= 0) {
-              reinterpret_cast<float4*>(p.part + (static_cast<long long>(to) * NR + r) * HD)[c] = o;
+              reinterpret_cast<float4*>(p.part + (static_cast<long long>(to) * kRows + r) * HD)[c] = o;
               if (c == 0) s_inv[r] = lse2;
             } else {
               const long long orow = static_cast<long long>(g.begin + g.i0 + r / p.group) * p.heads + g.head * p.group + r % p.group;
@@ -627,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           }
           if (to >= 0) {  // the group's log-sum-exps have been read: its first slot takes the joined ones
             softmax_sync();
-            if (t_key < g.rows) p.part_lse[to * NR + t_key] = s_inv[t_key];
+            if (t_key < g.rows) p.part_lse[to * kRows + t_key] = s_inv[t_key];
           }
           if (to < 0) break;
           base = 0;
@@ -647,32 +616,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
   }
 }
 
-template <typename T, int HD, int NR>
-cudaError_t launch(TreeParams& p, cudaStream_t stream) {
-  auto kern = tree_few_kernel<T, HD, NR>;
-  static std::atomic<bool> configured[kMaxFlagDevices];
-  const cudaError_t e = ensure_smem_limit(kern, Few<HD, NR>::kSmemBytes, configured);
-  if (e != cudaSuccess) return e;
-  return launch_pdl(kern, p.grid, kThreads, Few<HD, NR>::kSmemBytes, stream, p);
-}
-
 template <typename T, int HD>
-cudaError_t launch_rows(TreeParams& p, int rows, cudaStream_t stream) {
-  return launch<T, HD, 16>(p, stream);
+cudaError_t launch(TreeParams& p, cudaStream_t stream) {
+  auto kern = tree_few_kernel<T, HD>;
+  static std::atomic<bool> configured[kMaxFlagDevices];
+  const cudaError_t e = ensure_smem_limit(kern, Few<HD>::kSmemBytes, configured);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, p.grid, kThreads, Few<HD>::kSmemBytes, stream, p);
 }
 
 }  // namespace
 
-cudaError_t launch_tree_few(TreeParams& p, const fl_tree_attention_args& a, int rows, cudaStream_t stream) {
+cudaError_t launch_tree_few(TreeParams& p, const fl_tree_attention_args& a, cudaStream_t stream) {
   p.grid = kCtasPerSm * sm_count();
-  p.tile_tokens = rows / p.group;
-  p.part_lse = p.part + 2LL * p.grid * rows * a.head_dim;
-  p.arrived = reinterpret_cast<unsigned long long*>(p.part_lse + 2LL * p.grid * rows);
+  p.tile_tokens = kRows / p.group;
+  p.part_lse = p.part + 2LL * p.grid * kRows * a.head_dim;
+  p.arrived = reinterpret_cast<unsigned long long*>(p.part_lse + 2LL * p.grid * kRows);
   if (!encode_tree_maps(p, a, kBN)) return cudaErrorInvalidValue;
-  if (a.dtype == FL_DTYPE_F16)
-    return a.head_dim == 64 ? launch_rows<__half, 64>(p, rows, stream) : launch_rows<__half, 128>(p, rows, stream);
-  return a.head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(p, rows, stream)
-                          : launch_rows<__nv_bfloat16, 128>(p, rows, stream);
+  if (a.dtype == FL_DTYPE_F16) return a.head_dim == 64 ? launch<__half, 64>(p, stream) : launch<__half, 128>(p, stream);
+  return a.head_dim == 64 ? launch<__nv_bfloat16, 64>(p, stream) : launch<__nv_bfloat16, 128>(p, stream);
 }
 
 }  // namespace fl
