@@ -123,6 +123,10 @@ def build_binding(verbose: bool = False) -> Path:
            *[f"-L{p}" for p in libdirs], f"-L{PKG}",
            "-lflashlite_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
            "-ltorch_python", "-lcudart",
+           # torch's own C++ runtime, by file name: a compiler that finds only
+           # libstdc++.a would link a second one in, whose streams do not work
+           # with the first one's locales (a number in an error text crashes)
+           "-l:libstdc++.so.6",
            "-Wl,-rpath,$ORIGIN"]
     out = _run(cmd, BUILD / "binding.log")
     if verbose:

@@ -359,12 +359,12 @@ int rotary(const fl_rotary_args* args, void* stream) {
       a.head_dim > (1LL << 16))
     return fail(FL_ERR_INVALID_ARGUMENT, "dimension too large");
   if (a.batch == 0 || a.length == 0 || a.heads + a.kv_heads == 0) return FL_OK;
+  if (a.slots != nullptr && (a.page_size <= 0 || a.cache_blocks < 0))
+    return fail(FL_ERR_INVALID_ARGUMENT, "page_size must be positive");
   if ((a.heads > 0 && (!a.q || !a.q_out)) || (a.kv_heads > 0 && (!a.k || !a.k_out)) || (!a.table && a.rot > 0))
     return fail(FL_ERR_INVALID_ARGUMENT, "null tensor pointer");
   if ((a.slots != nullptr) != (a.v != nullptr) || (a.v != nullptr && !a.v_out))
     return fail(FL_ERR_INVALID_ARGUMENT, "the cache form takes v, its cache and the slots together");
-  if (a.slots != nullptr && (a.page_size <= 0 || a.cache_blocks < 0))
-    return fail(FL_ERR_INVALID_ARGUMENT, "page_size must be positive");
   int st = check_device();
   if (st != FL_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

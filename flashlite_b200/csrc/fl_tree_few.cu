@@ -121,6 +121,7 @@ __device__ __forceinline__ float warp_sums(float (&a)[kRows], int lane) {
   }
   return a[0] + __shfl_xor_sync(0xffffffffu, a[0], 1);
 }
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __grid_constant__ TreeParams p) {
   using C = Few<HD>;

@@ -33,6 +33,16 @@ def test_cpu_tensors_are_refused():
         fa.rotary(q, q, table, layout="hnd")
 
 
+def test_refusal_that_names_a_number():
+    """An error text with a number in it (a C++ stream of the binding); tensors without storage stand for CUDA ones."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        ints = torch.empty((1, 2), dtype=torch.int32, device="cuda:0")
+        with pytest.raises(RuntimeError, match=r"context_lens must have 1 dimension"):
+            fa.plan_cache_step(ints, ints, ints, ints, ints, ints, 2, 16)
+
+
 def test_table_arguments():
     from flashlite_b200.rotary import rotary_table
 
