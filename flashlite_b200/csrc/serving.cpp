@@ -31,7 +31,7 @@ void* stream_of(const Tensor& t) {
 // Outputs of a call: contiguous tensors one after the other in one allocation
 // on the current stream of the current device, taken from torch's caching
 // allocator directly. The calls of a serving step run for microseconds, and
-// torch::empty costs most of one: six outputs 8.6 us a call, this way 6.
+// torch::empty costs most of one: six outputs 8.6 us a call, this way 5.3.
 class Outputs {
  public:
   explicit Outputs(size_t bytes)
@@ -275,7 +275,8 @@ Tensor rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Te
 // Blocks, slots, positions and tree masks of one serving step.
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor> plan_cache_step(
     const Tensor& context_lens, const Tensor& cu_seqlens, const Tensor& block_table, const Tensor& held_blocks,
-    const Tensor& free_blocks, const Tensor& num_free, int64_t total_tokens, int64_t page_size, const OptTensor& parents, int64_t mask_words) {
+    const Tensor& free_blocks, const Tensor& num_free, int64_t total_tokens, int64_t page_size, const OptTensor& parents,
+    int64_t mask_words) {
   TORCH_CHECK(context_lens.is_cuda(), "All tensors must be on CUDA");
   const torch::Device dev = context_lens.device();
   check_ints(context_lens, dev, torch::kInt, 1, "context_lens");
