@@ -201,20 +201,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
       Segment g;
       if (worker == 0) {
         g = sched.next();
-        if (!wait_all(bar_segempty + 8 * sl, ((seg / kSegRing) & 1) ^ 1, abort_flag, p.err)) break;
-        if (lane == 0) {
-          segs[sl] = g;
-          mbar_arrive(bar_segfull + 8 * sl);
-        }
-        __syncwarp();
       } else {
         if (!wait_all(bar_segfull + 8 * sl, (seg / kSegRing) & 1, abort_flag, p.err)) break;
         g = segs[sl];
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_segempty + 8 * sl);
       }
+      PageNumbers<kBN> pages(p, g, lane);  // of none after the last segment
+      if (worker == 0) {
+        if (!wait_all(bar_segempty + 8 * sl, ((seg / kSegRing) & 1) ^ 1, abort_flag, p.err)) break;
+        if (lane == 0) {
+          segs[sl] = g;
+          mbar_arrive(bar_segfull + 8 * sl);
+        }
+        __syncwarp();
+      }
       if (g.t1 < 0) break;
-      PageNumbers<kBN> pages(p, g, lane);
       if (worker == 0) {
         if (!wait_all(bar_qfree + 8 * (seg & 1), ((seg >> 1) & 1) ^ 1, abort_flag, p.err)) break;
         if (lane == 0) {
@@ -420,13 +422,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           // new maxima: over the warp, then the four warps
 #pragma unroll
           for (int r = 0; r < kRows; ++r) {
+            if (r % 4 == 0 && r >= g.rows) break;  // four rows at a time: the others see nothing
             const float m = warp_max(y[r]);
             if (lane == 0) s_max[4 * r + (warp & 3)] = m;
           }
           softmax_sync();
           float alpha[kRows];
 #pragma unroll
+          for (int r = 0; r < kRows; ++r) alpha[r] = 1.0f;
+#pragma unroll
           for (int r = 0; r < kRows; ++r) {
+            if (r % 4 == 0 && r >= g.rows) break;
             const float4 w = reinterpret_cast<const float4*>(s_max)[r];
             const float m = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
             const float next = m - ref[r] > kLag + kUp ? m - kUp : ref[r];
@@ -479,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
         }
       }
       softmax_sync();
+      float lse2 = 0.0f;
       if (t_key < g.rows) {
         float sum = 0.0f, sum_r = 0.0f, m = 0.0f;
 #pragma unroll
@@ -489,14 +496,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
 #pragma unroll
         for (int r = 0; r < kRows; ++r) m = r == t_key ? ref[r] : m;
         s_inv[t_key] = sum == 0.0f ? 0.0f : 1.0f / sum_r;
-        const float lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
+        lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
+      }
+      softmax_sync();
+      if (t_key < g.rows) {
         if (g.slot >= 0)
           p.part_lse[g.slot * kRows + t_key] = lse2;
         else if (p.lse != nullptr)
           p.lse[static_cast<long long>(g.begin + g.i0 + t_key / p.group) * p.heads + g.head * p.group + t_key % p.group] =
               lse2 * 0.69314718055994531f;
       }
-      softmax_sync();
       ok = wait_all(bar_pv + 8 * ((js - 1) & 1), ((js - 1) >> 1) & 1, abort_flag, p.err) &&
            wait_all(bar_seg + 8 * (seg & 1), (seg >> 1) & 1, abort_flag, p.err);
       tc_fence_after();
@@ -565,7 +574,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           if (*last_flag == 0) break;
           const int to = stride == 1 && groups > 1 ? slot_of(first, base) : -1;
           constexpr int kVecs = HD / 4, kBatch = 9;
-          float lse2 = 0.0f;
 #pragma unroll 1
           for (int i = t_key; i < g.rows * kVecs; i += 128) {
             const int r = i / kVecs, c = i % kVecs;
