@@ -323,7 +323,8 @@ cudaError_t launch(const fl_rotary_args& a, cudaStream_t stream) {
   const int steps = (p.heads + hstep - 1) / hstep;
   const long long slots = static_cast<long long>(kBlocksPerSm) * sm_count() * (kThreads / 32);
   long long best = 0;
-  for (int n = 1; n <= std::min(steps, kMaxDivision); ++n) {
+  if (rows * steps <= slots) p.chunk = hstep;  // all in one wave
+  for (int n = 1; rows * steps > slots && n <= std::min(steps, kMaxDivision); ++n) {
     const long long per = (steps + n - 1) / n, waves = (rows * ((steps + per - 1) / per) + slots - 1) / slots;
     if (best == 0 || waves * (per + 4) < best) {
       best = waves * (per + 4);
