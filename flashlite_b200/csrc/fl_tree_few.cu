@@ -231,6 +231,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
       ++seg;
       for (int t = g.t0; ok && t < g.t1; ++t) {
         pages.begin_tile(t);
+        if (worker > 0 && pages.boxes(g, t) <= worker) {
+          // No box of the tile is this warp's: it comes and goes without it. A
+          // wait for its stage could find it used and freed already, and take
+          // the phase it waits for for one still to come.
+          n += 2;
+          continue;
+        }
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++n) {
           const int st = n % kStages;

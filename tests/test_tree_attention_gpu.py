@@ -222,6 +222,21 @@ def test_ragged_batches(cuda, dim, dtype, heads, tokens):
          poison=True).check()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 256])
+def test_caches_of_one_page_among_longer_ones(cuda, dim, page):
+    """Tiles of a single page, which one of two loading warps fetches alone, by the dozen in each CTA, then tiles of many:
+    the other warp must neither wait for what has come and gone nor miss its turn. Many runs, as it is a matter of time."""
+    rng = random.Random(page + dim)
+    lengths = [(rng.choice([3, 9, 15, 15, 15, 900]), 1) for _ in range(900)]
+    c = Case(cuda, lengths, 4, 4, dim, page)
+    first = c.check()
+    for _ in range(100):
+        again = c.run()
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    assert fa.device_error() == 0
+
+
 def test_repeatable(cuda):
     """The same bits every time: no sum depends on the order in which parts finish."""
     c = Case(cuda, [(9000, 4), (501, 4), (33, 4)], 8, 2, 128, 16)
