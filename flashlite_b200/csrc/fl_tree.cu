@@ -53,6 +53,10 @@ constexpr int kCtasPerSm = 2;
 // (tree of 61 nodes x 4 heads: 99 -> 89 us); with few rows the look costs more
 // than the part (3 us on the smallest calls).
 constexpr int kDirectRows = 32;
+// What a change of units costs in tiles: of 0, 2, 3, 4, 6, 8 and 12, 3 is best
+// or within 2 % of it (40 requests x 8 tokens over 6000 keys 105 us for 110,
+// 4 prompts of 1000 38 for 42, chunks 258 for 270).
+constexpr int kGapTiles = 3;
 
 // Shape per head dimension; tiles are made of 64-column (128-byte) swizzle
 // atoms as in the other forward kernels. K and V tiles are 16 KB both ways;
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsProducer<HD>));
     if (warp == 3) {
       // ======================= scheduler =======================
-      Scheduler<kBN, kAligned> sched(p, cta, lane);
+      Scheduler<kBN, kAligned, kGapTiles> sched(p, cta, lane);
       for (int ring = 0;; ++ring) {
         const Segment g = sched.next();
         const int st = ring % kSegRing;

@@ -105,14 +105,15 @@ __device__ __forceinline__ int tiles_of(const TreeParams& p, const Request& r, i
   return max(1, (keys_of(p, r, i0) + kBN - 1) / kBN);
 }
 
-// Tiles of one key head of a request: those of all its row tiles.
+// Tiles of one key head of a request: those of all its row tiles, and `gap`
+// more for each.
 template <int kBN>
-__device__ __forceinline__ long long head_tiles(const TreeParams& p, const Request& r) {
+__device__ __forceinline__ long long head_tiles(const TreeParams& p, const Request& r, int gap) {
   if (r.count == 0) return 0;
   if (p.mask != nullptr)
-    return static_cast<long long>((r.count + p.tile_tokens - 1) / p.tile_tokens) * tiles_of<kBN>(p, r, 0);
+    return static_cast<long long>((r.count + p.tile_tokens - 1) / p.tile_tokens) * (tiles_of<kBN>(p, r, 0) + gap);
   long long n = 0;
-  for (int i0 = 0; i0 < r.count; i0 += p.tile_tokens) n += tiles_of<kBN>(p, r, i0);
+  for (int i0 = 0; i0 < r.count; i0 += p.tile_tokens) n += tiles_of<kBN>(p, r, i0) + gap;
   return n;
 }
 
@@ -165,7 +166,10 @@ struct Segment {
 // of up to 4096 keys: 16.7 us for 22.1, few cuts against many).
 constexpr int kWholeTiles = 3, kShortPart = 8;
 
-template <int kBN, bool kAligned>
+//
+// kGap: the tiles that a change of units costs a CTA. Units are divided as if
+// they began with so many more, so that CTAs with more units get fewer tiles.
+template <int kBN, bool kAligned, int kGap>
 struct Scheduler {
   const TreeParams& p;
   const int cta, lane;
@@ -191,7 +195,7 @@ struct Scheduler {
     const int b0 = min(lane * per, p.requests), b1 = min(b0 + per, p.requests);
     long long mine = 0;
     if (per <= 1) {
-      if (lane < p.requests) mine = p.kv_heads * head_tiles<kBN>(p, request_of(p, l_begin, l_end, l_ctx, cta == 0));
+      if (lane < p.requests) mine = p.kv_heads * head_tiles<kBN>(p, request_of(p, l_begin, l_end, l_ctx, cta == 0), kGap);
     } else {
       for (int x = b0; x < b1; ++x) mine += tiles(x, cta == 0);
     }
@@ -248,7 +252,7 @@ struct Scheduler {
     const int units = __reduce_add_sync(0xffffffffu, row_tiles) * p.kv_heads;
     if (units >= p.grid) return false;
     const int first_tiles = tiles_of<kBN>(p, mine, 0);
-    const long long tiles = one ? row_tiles * first_tiles : head_tiles<kBN>(p, mine);
+    const long long tiles = one ? row_tiles * first_tiles : head_tiles<kBN>(p, mine, 0);
     if (__any_sync(0xffffffffu, tiles > 1 << 15)) return false;
     const int total = __reduce_add_sync(0xffffffffu, static_cast<int>(tiles)) * p.kv_heads;
     const int spare = p.grid - units;  // sum of ceil(n / part_tiles) <= grid
@@ -316,17 +320,17 @@ struct Scheduler {
                        __shfl_sync(0xffffffffu, l_ctx, b - base), false);
         h = i0 = 0;
         if (off > 0) {  // the share begins inside this request
-          const long long per_head = head_tiles<kBN>(p, r);
+          const long long per_head = head_tiles<kBN>(p, r, kGap);
           h = static_cast<int>(divide(off, per_head));
           off -= h * per_head;
           if (p.mask != nullptr) {
-            const int n = tiles_of<kBN>(p, r, 0), rt = static_cast<int>(divide(off, n));
+            const int n = tiles_of<kBN>(p, r, 0) + kGap, rt = static_cast<int>(divide(off, n));
             i0 = rt * p.tile_tokens;
             off -= static_cast<long long>(rt) * n;
           } else {  // 32 row tiles at a time
             while (true) {
               const int mine = i0 + lane * p.tile_tokens;
-              int upto = mine < r.count ? tiles_of<kBN>(p, r, mine) : 0;
+              int upto = mine < r.count ? tiles_of<kBN>(p, r, mine) + kGap : 0;
 #pragma unroll
               for (int d = 1; d < 32; d <<= 1) {
                 const int x = __shfl_up_sync(0xffffffffu, upto, d);
@@ -351,19 +355,25 @@ struct Scheduler {
       entered = false;
     }
     const int n = tiles_of<kBN>(p, r, i0);
+    g.t0 = max(static_cast<int>(off) - kGap, 0);
+    const int t1 = static_cast<int>(min(static_cast<long long>(n), off + (s1 - s) - kGap));
+    if (kGap > 0 && t1 <= g.t0) {  // the share ends before the unit's first tile
+      s = s1;
+      return g;
+    }
+    g.t1 = t1;
     fill(g);
-    g.t0 = static_cast<int>(off);
-    g.t1 = static_cast<int>(min(static_cast<long long>(n), off + (s1 - s)));
     const bool whole = g.t0 == 0 && g.t1 == n;
     g.slot = whole ? -1 : 2 * cta + (g.t0 == 0 ? 1 : 0);
     g.part = 0;
     g.parts = 1;
     if (!whole) {
-      const int first = div.owner(s - off);
+      const long long tile0 = s - off + kGap;
+      const int first = div.owner(tile0);
       g.part = cta - first;
-      g.parts = div.owner(s - off + n - 1) - first + 1;
+      g.parts = div.owner(tile0 + n - 1) - first + 1;
     }
-    s += g.t1 - g.t0;
+    s += g.t1 + kGap - off;
     off = 0;
     i0 += p.tile_tokens;
     return g;
@@ -390,7 +400,7 @@ struct Scheduler {
     }
   }
   __device__ __forceinline__ long long tiles(int x, bool report) const {
-    return p.kv_heads * head_tiles<kBN>(p, request_of(p, p.cu[x], p.cu[x + 1], p.context[x], report));
+    return p.kv_heads * head_tiles<kBN>(p, request_of(p, p.cu[x], p.cu[x + 1], p.context[x], report), kGap);
   }
 };
 

@@ -39,6 +39,7 @@ constexpr int kRows = kFewRows;  // rows per unit (UMMA N): a P^T row is 32 byte
 static_assert(kRows == 16, "one 32-byte swizzle atom");
 constexpr int kCtasPerSm = 2;
 constexpr int kProducers = 2;  // warps 0 and 3
+constexpr int kGapTiles = 2;   // what a change of units costs (256 requests of 500 keys: 84 us, 93 with none)
 // Register split: 128 x 112 (producers, MMA) + 128 x 144 (softmax) = 256 x 128, the launch's total.
 constexpr int kRegsProducer = 112, kRegsSoftmax = 144;
 
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
     // ======================= producers; warp 0 is the scheduler too =======================
     // (Between a launch and its first load there is no hand-over.)
     const int worker = warp == 0 ? 0 : 1;
-    Scheduler<kBN, true> sched(p, cta, lane, warp == 0);
+    Scheduler<kBN, true, kGapTiles> sched(p, cta, lane, warp == 0);
     int n = 0, seg = 0;  // tiles of K and V, and Q tiles, so far
     bool ok = true;
     while (ok) {
