@@ -129,7 +129,6 @@ __device__ __forceinline__ long long row_of(const int64_t (&st)[3], long long b,
 template <typename T, int VEC, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_kernel(const __grid_constant__ RotaryParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t w = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (w >= p.warps) return;
   const fl_rotary_args& a = p.a;
@@ -143,6 +142,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_kernel(const __
   const int hstep = p.over_heads ? groups : 1;
   const int hq = static_cast<int>(a.heads), hk = static_cast<int>(a.kv_heads);
   const int h0 = chunk * p.chunk;
+  const T* q_in = static_cast<const T*>(a.q) + row_of(a.q_stride, b, n, 0);
+  const T* k_in = static_cast<const T*>(a.k) + row_of(a.k_stride, b, n, 0);
+  const T* v_in = static_cast<const T*>(a.v) + row_of(a.v_stride, b, n, 0);
+  T* q_out = static_cast<T*>(a.q_out) + row_of(a.q_out_stride, b, n, 0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const uint32_t pi = a.positions_batch ? t : n;
   const long long pos = a.positions == nullptr ? n
@@ -167,10 +171,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_kernel(const __
     }
   }
 
-  const T* q_in = static_cast<const T*>(a.q) + row_of(a.q_stride, b, n, 0);
-  const T* k_in = static_cast<const T*>(a.k) + row_of(a.k_stride, b, n, 0);
-  const T* v_in = static_cast<const T*>(a.v) + row_of(a.v_stride, b, n, 0);
-  T* q_out = static_cast<T*>(a.q_out) + row_of(a.q_out_stride, b, n, 0);
   T* k_out = static_cast<T*>(a.k_out) + (a.slots == nullptr ? row_of(a.k_out_stride, b, n, 0) : kc);
   T* v_out = static_cast<T*>(a.v_out) + vc;
   // a token without a slot has only its q heads
