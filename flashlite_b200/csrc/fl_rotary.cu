@@ -13,8 +13,8 @@
 // 16-byte vectors of a row and walks over a token's heads with their cosines
 // and sines in registers, so the table is read once per token and warp, not
 // once per head. The lanes of a warp that the columns of one row leave over
-// take further heads where heads are closer together in memory than tokens,
-// further tokens otherwise. What it takes is bytes under way: through
+// take further heads where heads are closer together in memory than tokens and
+// many enough, further tokens otherwise. What it takes is bytes under way: through
 // registers, two heads at a time at 24 warps per SM, a training step's q and
 // k of 1 GB ran at 5.1 TB/s; with asynchronous copies into slots of shared
 // memory that are each thread's own, four heads ahead, at 6.6 TB/s (153 us
@@ -310,7 +310,11 @@ cudaError_t launch(const fl_rotary_args& a, cudaStream_t stream) {
   const int groups = 32 / p.lanes;
   p.heads = static_cast<int>(a.heads + a.kv_heads * (a.v != nullptr ? 2 : 1));
   const int64_t(&near)[3] = a.heads > 0 ? a.q_stride : a.k_stride;
-  p.over_heads = near[2] <= near[1] ? 1 : 0;
+  // Heads side by side where they are closer together than tokens and leave a
+  // warp at least as many steps as it has copies under way; with fewer it
+  // mostly starts and ends (4 x 8192 tokens of 16 + 4 heads of 64, 2.5 steps:
+  // 35.5 us, 31.2 with tokens side by side; of 32 + 8 heads, 5 steps: 30.2, 31.4).
+  p.over_heads = near[2] <= near[1] && p.heads >= kDepth * groups ? 1 : 0;
   const long long tokens = a.batch * a.length;
   const long long rows = p.over_heads ? tokens : (tokens + groups - 1) / groups;
   // The heads of a token are divided among warps so that the last wave of
