@@ -189,6 +189,20 @@ def test_append(cuda, dtype, layout, shape):
     assert fa.device_error() == 0
 
 
+@pytest.mark.parametrize("shape", [(2, 67, 2, 1, 64, 64), (1, 9, 32, 8, 64, 64), (3, 70, 16, 4, 64, 32), (1, 21, 8, 2, 128, 128),
+                                   (2, 300, 3, 1, 64, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_divisions(cuda, interleaved, shape):
+    """Few heads and many, in odd numbers of tokens: tokens or heads side by side, one or more parts to a token."""
+    test_rotary_matches_the_formula(cuda, torch.bfloat16, "bnhd", interleaved, shape)
+
+
+@pytest.mark.parametrize("shape", [(11, 32, 8, 64, 64, 16, False), (6, 16, 4, 128, 128, 8, True), (131, 2, 1, 64, 64, 16, False),
+                                   (50, 40, 40, 64, 32, 8, False)])
+def test_append_divisions(cuda, shape):
+    test_append(cuda, torch.float16, "bnhd", shape)
+
+
 def test_append_slot_out_of_range(cuda):
     q = torch.randn(3, 2, 64, device=cuda).half()
     kc = torch.zeros(2, 8, 2, 64, device=cuda).half()
