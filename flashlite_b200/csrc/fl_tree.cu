@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       // while the CTA of its first part is still at work.
       const int first = cta - g.part;
       bool direct = false;
-      if (g.slot >= 0 && g.parts <= kJoinGroup && g.rows > kDirectRows) {
+      if (g.slot >= 0 && g.parts <= kJoinMany && g.rows > kDirectRows) {
         if (t_row == 0)
           *last_flag = mbar_wait(bar_count + 8 * (g.slot & 1), 0, abort_flag, p.err) &&
                        others_arrived(group_word(p, g, cta), p.tag, g.parts);
@@ -671,8 +671,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       ++seg;
       if (g.slot >= 0 && !direct) {
         // a part: whoever arrives last joins, within its group of parts and then among the groups
-        const int groups = (g.parts + kJoinGroup - 1) / kJoinGroup;
-        int base = g.part / kJoinGroup * kJoinGroup, stride = 1, n = min(kJoinGroup, g.parts - base);
+        const int size = join_group(g), groups = g.parts <= size ? 1 : (g.parts + size - 1) / size;
+        int base = group_base(g, size), stride = 1, n = min(size, g.parts - base);
 #pragma unroll 1
         while (true) {
           if (!(ok = meet())) break;  // all of this CTA's part is written
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
           if (!(ok = meet())) break;  // the group's log-sum-exps have been read: its first slot takes the joined ones
           if (live) p.part_lse[to * kBM + t_row] = lse2;
           base = 0;
-          stride = kJoinGroup;
+          stride = size;
           n = groups;
         }
       }

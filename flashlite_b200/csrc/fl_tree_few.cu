@@ -569,8 +569,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
       if (g.slot >= 0) {
         // a part: whoever arrives last joins, within its group of parts and then among the groups:
         //   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M),  M = max_k lse_k
-        const int first = cta - g.part, groups = (g.parts + kJoinGroup - 1) / kJoinGroup;
-        int base = g.part / kJoinGroup * kJoinGroup, stride = 1, n = min(kJoinGroup, g.parts - base);
+        const int first = cta - g.part, groups = (g.parts + kJoinFew - 1) / kJoinFew;
+        int base = group_base(g, kJoinFew), stride = 1, n = min(kJoinFew, g.parts - base);
 #pragma unroll 1
         while (true) {
           __syncwarp();
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           }
           if (to < 0) break;
           base = 0;
-          stride = kJoinGroup;
+          stride = kJoinFew;
           n = groups;
         }
       }
