@@ -20,9 +20,9 @@
 // multiplications 256: every instruction reads its 128 rows of Q from shared
 // memory again, 67 cycles for 64 keys and 79 for 128), P V 400, softmax 1,550
 // with both CTAs' warps at work. 4 requests of 509 tokens x 4 heads to a key
-// head over up to 8192 keys, bf16: 258 to 277 us, 740 to 790 TFLOP/s, at some
+// head over up to 8192 keys, bf16: 258 to 283 us, 720 to 790 TFLOP/s, at some
 // 1.4 GHz under the power limit; 16 trees of 61 nodes x 4 heads over up to
-// 5000 keys: 77 to 94 us, with 6 us to the first tile. Half of Q kept in TMEM
+// 5000 keys: 76 to 94 us, with 6 us to the first tile. Half of Q kept in TMEM
 // took 9 % off a tile's cycles and nothing off the time. Two row tiles in one
 // CTA per SM, with K and V read once for both, were slower: TMEM then holds S
 // of 128 keys only with P in its place, which puts S, softmax and P V in a
