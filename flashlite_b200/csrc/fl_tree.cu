@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
         __syncwarp();
         if (g.t1 < 0) break;
         if (g.slot >= 0) {
-          ready_counts(p, g, cta, lane);
+          ready_counts(p, g, cta, lane, join_group(g));
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_count + 8 * (g.slot & 1));
         }
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       if (g.slot >= 0 && g.parts <= kJoinMany && g.rows > kDirectRows) {
         if (t_row == 0)
           *last_flag = mbar_wait(bar_count + 8 * (g.slot & 1), 0, abort_flag, p.err) &&
-                       others_arrived(group_word(p, g, cta), p.tag, g.parts);
+                       others_arrived(group_word(p, g, cta, kJoinMany), p.tag, g.parts);
         if (!(ok = meet())) break;
         direct = *last_flag != 0;
       }
@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
           if (!(ok = meet())) break;  // all of this CTA's part is written
           if (t_row == 0)
             *last_flag = mbar_wait(bar_count + 8 * (g.slot & 1), 0, abort_flag, p.err) &&
-                         arrive_last(stride == 1 ? group_word(p, g, cta) : unit_word(p, g, cta), n);
+                         arrive_last(stride == 1 ? group_word(p, g, cta, size) : unit_word(p, g, cta), n);
           if (!(ok = meet())) break;
           if (*last_flag == 0) break;
           const int to = stride == 1 && groups > 1 ? slot_of(first, base) : -1;

@@ -566,16 +566,16 @@ __device__ __forceinline__ int join_group(const Segment& g) {
 // the first arrival). The last arrival clears the word, for a captured call
 // that runs again with the same tag.
 __device__ __forceinline__ int slot_of(int first, int part) { return part == 0 ? 2 * first + 1 : 2 * (first + part); }
-__device__ __forceinline__ unsigned long long* group_word(const TreeParams& p, const Segment& g, int cta) {
-  return p.arrived + slot_of(cta - g.part, group_base(g, join_group(g)));
+__device__ __forceinline__ unsigned long long* group_word(const TreeParams& p, const Segment& g, int cta, int size) {
+  return p.arrived + slot_of(cta - g.part, group_base(g, size));
 }
 __device__ __forceinline__ unsigned long long* unit_word(const TreeParams& p, const Segment& g, int cta) {
   return p.arrived + 2 * p.grid + (cta - g.part);
 }
 // By the first two lanes of the scheduler warp, for a part g of CTA cta.
-__device__ __forceinline__ void ready_counts(const TreeParams& p, const Segment& g, int cta, int lane) {
+__device__ __forceinline__ void ready_counts(const TreeParams& p, const Segment& g, int cta, int lane, int size) {
   if (lane >= 2) return;
-  unsigned long long* word = lane == 0 ? group_word(p, g, cta) : unit_word(p, g, cta);
+  unsigned long long* word = lane == 0 ? group_word(p, g, cta, size) : unit_word(p, g, cta);
   const unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(word);
   if ((seen >> 16) != p.tag) atomicCAS(word, seen, p.tag << 16);
 }

@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
                              kProducers, kv == 0);
         }
         if (worker == 0 && t == g.t0 && g.slot >= 0) {  // while the first tile is on its way
-          ready_counts(p, g, cta, lane);
+          ready_counts(p, g, cta, lane, kJoinFew);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_count + 8 * (g.slot & 1));
         }
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           if (softmax_any(!ok)) break;  // otherwise all of this CTA's part is written
           if (t_key == 0)
             *last_flag = mbar_wait(bar_count + 8 * (g.slot & 1), 0, abort_flag, p.err) &&
-                         arrive_last(stride == 1 ? group_word(p, g, cta) : unit_word(p, g, cta), n);
+                         arrive_last(stride == 1 ? group_word(p, g, cta, kJoinFew) : unit_word(p, g, cta), n);
           softmax_sync();
           if (*last_flag == 0) break;
           const int to = stride == 1 && groups > 1 ? slot_of(first, base) : -1;
