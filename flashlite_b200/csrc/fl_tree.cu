@@ -184,7 +184,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + kFlagOff + 4);
   volatile int* bad_flag = reinterpret_cast<volatile int*>(misc + kFlagOff + 8);
   volatile int* last_flag = reinterpret_cast<volatile int*>(misc + kFlagOff + 12);
-  static_assert(kFlagOff + 16 <= 1024, "misc block");
+  // One word for each of the CTA's (up to) two parts: the first softmax warp can
+  // be at the second part's decision while another has yet to read the first
+  // part's, which a meeting's end does not hold it back from.
+  volatile int* direct_flag = reinterpret_cast<volatile int*>(misc + kFlagOff + 16);
+  static_assert(kFlagOff + 24 <= 1024, "misc block");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x;
@@ -572,10 +576,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
       bool direct = false;
       if (g.slot >= 0 && g.parts <= kJoinMany && g.rows > kDirectRows) {
         if (t_row == 0)
-          *last_flag = mbar_wait(bar_count + 8 * (g.slot & 1), 0, abort_flag, p.err) &&
-                       others_arrived(group_word(p, g, cta, kJoinMany), p.tag, g.parts);
+          direct_flag[g.slot & 1] = mbar_wait(bar_count + 8 * (g.slot & 1), 0, abort_flag, p.err) &&
+                                    others_arrived(group_word(p, g, cta, kJoinMany), p.tag, g.parts);
         if (!(ok = meet())) break;
-        direct = *last_flag != 0;
+        direct = direct_flag[g.slot & 1] != 0;
       }
 
       // ---- epilogue of the segment ----
