@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
     // (Between a launch and its first load there is no hand-over.)
     const int worker = warp == 0 ? 0 : 1;
     Scheduler<kBN, true, kGapTiles> sched(p, cta, lane, warp == 0);
-    int n = 0, seg = 0;  // tiles of K and V, and Q tiles, so far
+    int n = 0, seg = 0;   // tiles of K and V, and Q tiles, so far
+    uint32_t issued = 0;  // bit i: this warp has copies in tile n - 1 - i
     bool ok = true;
     while (ok) {
       const int sl = seg % kSegRing;
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           // wait for its stage could find it used and freed already, and take
           // the phase it waits for for one still to come.
           n += 2;
+          issued <<= 2;
           continue;
         }
 #pragma unroll
@@ -248,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
           }
           load_tile<HD, kBN>(p, kv ? &p.tm_v : &p.tm_k, pages, g, t, sbase + st * C::kTileBytes, C::full(bar_full, n), worker,
                              kProducers, kv == 0);
+          issued = issued << 1 | 1u;
         }
         if (worker == 0 && t == g.t0 && g.slot >= 0) {  // while the first tile is on its way
           ready_counts(p, g, cta, lane, kJoinFew);
@@ -256,10 +259,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
         }
       }
     }
-    if (*abort_flag && lane == 0 && worker == 0) {
-      // let every copy under way land before shared memory is released
-      for (int i = max(n - kStages, 0); i < n; ++i) mbar_wait_quiet(C::full(bar_full, i), C::full_phase(i));
-      for (int i = max(seg - 2, 0); i < seg; ++i) mbar_wait_quiet(bar_qfull + 8 * (i & 1), (i >> 1) & 1);
+    if (*abort_flag && lane == 0) {
+      // Let every copy that this warp started land before shared memory is
+      // released. A stage is loaded anew only after its tile has come, but the
+      // second warp may have skipped a tile (two of the stream) that the first
+      // has yet to load.
+      constexpr int kUnderWay = kStages + 2;
+      static_assert(kUnderWay <= 32, "a bit for each");
+      for (int i = max(n - kUnderWay, 0); i < n; ++i)
+        if (issued >> (n - 1 - i) & 1u) mbar_wait_quiet(C::full(bar_full, i), C::full_phase(i));
+      if (worker == 0)
+        for (int i = max(seg - 2, 0); i < seg; ++i) mbar_wait_quiet(bar_qfull + 8 * (i & 1), (i >> 1) & 1);
     }
   } else if (warp == 1) {
     // ======================= S^T = K Q^T =======================
