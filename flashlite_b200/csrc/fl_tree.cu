@@ -92,23 +92,23 @@ template <int HD>
 constexpr int kRegsSoftmax = 256 - kRegsProducer<HD>;
 
 // Joins the n partial results base, base + stride, ... of a unit:
-//   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M),  M = max_k lse_k,
+//   o = sum_k l_k 2^(m_k - M) o_k / sum_k l_k 2^(m_k - M),  M = max_k m_k,
 // by the 128 softmax threads; into slot `to` or, if to < 0, out. Part i of a
 // unit that begins in CTA `first` is slot 2 first + 1 (i = 0) or 2 (first + i).
 // Neighbouring threads take neighbouring rows (the layout of a slot is
 // [D / 4][128] float4), and the columns that few rows leave threads for.
-// Returns the joined log2-sum-exp of row tid, if tid < rows.
+// Returns the joined reference and sum of row tid, if tid < rows.
 template <typename T, int HD>
-__device__ __forceinline__ float join_parts(const TreeParams& p, const Segment& g, int tid, int first, int base, int stride,
+__device__ __forceinline__ float2 join_parts(const TreeParams& p, const Segment& g, int tid, int first, int base, int stride,
                                             int n, int to) {
   constexpr int kVecs = HD / 4;
   int span = 1;  // rows, as a power of two
   while (span < g.rows) span *= 2;
   const int row = tid & (span - 1), lanes = kBM / span, c0 = tid / span;
-  if (row >= g.rows || c0 >= kVecs) return 0.0f;
+  if (row >= g.rows || c0 >= kVecs) return make_float2(0.0f, 0.0f);
   const int token = g.begin + g.i0 + row / p.group, head = g.head * p.group + row % p.group;
   const long long orow = static_cast<long long>(token) * p.heads + head;
-  float lse2 = 0.0f;
+  float2 joined = make_float2(-INFINITY, 0.0f);
   // kCols columns (of four) of kBatch parts at a time, all their loads under
   // way together. Rolled otherwise: on its first run in a kernel, code costs
   // as much to fetch as to execute.
@@ -121,12 +121,13 @@ __device__ __forceinline__ float join_parts(const TreeParams& p, const Segment& 
       for (int j = 0; j < 4 * kCols; ++j) acc[j] = 0.0f;
 #pragma unroll 1
       for (int k0 = 0; k0 < n; k0 += kBatch) {
-        float l[kBatch], v[kBatch][4 * kCols];
+        float2 l[kBatch];
+        float v[kBatch][4 * kCols];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const bool in = k0 + k < n;
           const int sl = slot_of(first, base + min(k0 + k, n - 1) * stride);
-          l[k] = in ? __ldcg(p.part_lse + sl * kBM + row) : -INFINITY;
+          l[k] = in ? __ldcg(p.part_sum + sl * kBM + row) : make_float2(-INFINITY, 0.0f);
           const float4* from = reinterpret_cast<const float4*>(p.part) + static_cast<long long>(sl) * kVecs * kBM + row;
 #pragma unroll
           for (int j = 0; j < kCols; ++j)
@@ -136,7 +137,7 @@ __device__ __forceinline__ float join_parts(const TreeParams& p, const Segment& 
         join_step<kBatch, 4 * kCols>(m, sum, acc, l, v);
       }
       const float inv = join_inv(sum);
-      lse2 = join_lse(m, sum);
+      joined = make_float2(m, sum);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) {
         if (c + j * lanes >= kVecs) break;
@@ -152,8 +153,8 @@ __device__ __forceinline__ float join_parts(const TreeParams& p, const Segment& 
   static_assert(kDirectRows >= 32, "units that are joined from registers take the first form");
   if (lanes * 4 <= kVecs) join(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
   else join(std::integral_constant<int, 1>{}, std::integral_constant<int, 6>{});
-  if (c0 == 0 && to < 0 && p.lse != nullptr) p.lse[orow] = lse2 * 0.69314718055994531f;
-  return lse2;
+  if (c0 == 0 && to < 0 && p.lse != nullptr) p.lse[orow] = join_lse(joined.x, joined.y) * 0.69314718055994531f;
+  return joined;
 }
 
 template <typename T, int HD, bool kAligned>
@@ -596,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
                            ? nullptr
                            : reinterpret_cast<float4*>(p.part) + static_cast<long long>(g.slot) * (HD / 4) * kBM + t_row;
         if (live) {
-          if (prow != nullptr) p.part_lse[g.slot * kBM + t_row] = lse2;
+          if (prow != nullptr) p.part_sum[g.slot * kBM + t_row] = make_float2(m_ref - kUp, l);
           else if (!direct && p.lse != nullptr) p.lse[orow] = lse2 * 0.69314718055994531f;
         }
 #pragma unroll 1
@@ -633,12 +634,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
             for (int c = 0; c < 32; ++c) acc[c] = 0.0f;
 #pragma unroll 1
             for (int k0 = 0; k0 < g.parts; k0 += 2) {
-              float l2[2], v[2][32];
+              float2 l2[2];
+              float v[2][32];
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 const bool in = k0 + k < g.parts, mine = k0 + k == g.part;
                 const int sl = slot_of(first, min(k0 + k, g.parts - 1));
-                l2[k] = !in ? -INFINITY : mine ? lse2 : __ldcg(p.part_lse + sl * kBM + t_row);
+                l2[k] = !in    ? make_float2(-INFINITY, 0.0f)
+                        : mine ? make_float2(m_ref - kUp, l)
+                               : __ldcg(p.part_sum + sl * kBM + t_row);
                 const float4* from = reinterpret_cast<const float4*>(p.part) +
                                      (static_cast<long long>(sl) * (HD / 4) + 8 * h) * kBM + t_row;
 #pragma unroll
@@ -686,10 +690,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
           if (!(ok = meet())) break;
           if (*last_flag == 0) break;
           const int to = stride == 1 && groups > 1 ? slot_of(first, base) : -1;
-          const float lse2 = join_parts<T, HD>(p, g, t_row, first, base, stride, n, to);
+          const float2 joined = join_parts<T, HD>(p, g, t_row, first, base, stride, n, to);
           if (to < 0) break;
-          if (!(ok = meet())) break;  // the group's log-sum-exps have been read: its first slot takes the joined ones
-          if (live) p.part_lse[to * kBM + t_row] = lse2;
+          if (!(ok = meet())) break;  // the group's sums have been read: its first slot takes the joined ones
+          if (live) p.part_sum[to * kBM + t_row] = joined;
           base = 0;
           stride = size;
           n = groups;
@@ -712,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
 // ---------------------------------------------------------------------------
 size_t workspace_bytes(int grid, int64_t head_dim) {
   const size_t slots = 2 * static_cast<size_t>(grid);
-  return slots * kBM * (head_dim + 1) * sizeof(float) + 3 * grid * sizeof(unsigned long long);
+  return slots * kBM * (head_dim + 2) * sizeof(float) + 3 * grid * sizeof(unsigned long long);
 }
 
 bool encode(CUtensorMap* tm, bool bf16, const void* base, int rank, const cuuint64_t* dims, const int64_t* strides,
@@ -741,8 +745,8 @@ template <typename T, int HD>
 cudaError_t launch(TreeParams& p, const fl_tree_attention_args& a, int64_t rows, cudaStream_t stream) {
   p.grid = kCtasPerSm * sm_count();
   p.tile_tokens = kBM / p.group;
-  p.part_lse = p.part + 2LL * p.grid * kBM * HD;
-  p.arrived = reinterpret_cast<unsigned long long*>(p.part_lse + 2LL * p.grid * kBM);
+  p.part_sum = reinterpret_cast<float2*>(p.part + 2LL * p.grid * kBM * HD);
+  p.arrived = reinterpret_cast<unsigned long long*>(p.part_sum + 2LL * p.grid * kBM);
   if (!encode_tree_maps(p, a, Shape<HD>::kBN)) return cudaErrorInvalidValue;
   // The aligned division pays where units are few (16 requests x 8 tokens x 2
   // key heads over 2000 keys, head dimension 128: 17.6 us for 22.1); elsewhere

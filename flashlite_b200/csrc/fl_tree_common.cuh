@@ -40,7 +40,7 @@ struct TreeParams {
   const int32_t* cu;
   const uint32_t* mask;
   float* part;      // partial results, 2 * grid slots: CTA c's are 2c (a unit's later part) and 2c + 1 (its first)
-  float* part_lse;  // their log2-sum-exp, a tile's rows for each slot
+  float2* part_sum; // their reference maximum (log2) and sum relative to it, a tile's rows for each slot
   unsigned long long* arrived;  // [2 * grid] by group of parts, [grid] by unit: tag and count
   unsigned long long tag;       // 48 bits, another one for each call
   unsigned int* err;
@@ -588,13 +588,15 @@ __device__ __forceinline__ bool arrive_last(unsigned long long* word, int n) {
 }
 
 // One step of a join, a running maximum over parts taken two (or more) at a
-// time: acc, sum and m take in parts with log2-sum-exps l and values v.
+// time: acc, sum and m take in parts with references l.x, sums l.y and values v.
+// (A part's log2-sum-exp in the place of the two would lose the sum where
+// scores are large: at 2^24 parts of 64 keys and of 1 would weigh the same.)
 template <int kBatch, int kVals>
-__device__ __forceinline__ void join_step(float& m, float& sum, float (&acc)[kVals], const float (&l)[kBatch],
+__device__ __forceinline__ void join_step(float& m, float& sum, float (&acc)[kVals], const float2 (&l)[kBatch],
                                           const float (&v)[kBatch][kVals]) {
   float m_new = m;
 #pragma unroll
-  for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, l[k]);
+  for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, l[k].x);
   const float m_use = m_new == -INFINITY ? 0.0f : m_new, alpha = ex2_approx(m - m_use);
   m = m_new;
   sum *= alpha;
@@ -602,7 +604,7 @@ __device__ __forceinline__ void join_step(float& m, float& sum, float (&acc)[kVa
   for (int j = 0; j < kVals; ++j) acc[j] *= alpha;
 #pragma unroll
   for (int k = 0; k < kBatch; ++k) {
-    const float w = ex2_approx(l[k] - m_use);
+    const float w = ex2_approx(l[k].x - m_use) * l[k].y;
     sum += w;
 #pragma unroll
     for (int j = 0; j < kVals; ++j) acc[j] = fmaf(w, v[k][j], acc[j]);

@@ -503,9 +503,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
         }
       }
       softmax_sync();
-      float lse2 = 0.0f;
+      float sum = 0.0f, m = 0.0f;
       if (t_key < g.rows) {
-        float sum = 0.0f, sum_r = 0.0f, m = 0.0f;
+        float sum_r = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           sum += s_sum[(w * kRows + t_key) * 2];
@@ -514,15 +514,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
 #pragma unroll
         for (int r = 0; r < kRows; ++r) m = r == t_key ? ref[r] : m;
         s_inv[t_key] = sum == 0.0f ? 0.0f : 1.0f / sum_r;
-        lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
       }
       softmax_sync();
       if (t_key < g.rows) {
         if (g.slot >= 0)
-          p.part_lse[g.slot * kRows + t_key] = lse2;
+          p.part_sum[g.slot * kRows + t_key] = make_float2(m, sum);
         else if (p.lse != nullptr)
           p.lse[static_cast<long long>(g.begin + g.i0 + t_key / p.group) * p.heads + g.head * p.group + t_key % p.group] =
-              lse2 * 0.69314718055994531f;
+              join_lse(m, sum) * 0.69314718055994531f;
       }
       ok = wait_all(bar_pv + 8 * ((js - 1) & 1), ((js - 1) >> 1) & 1, abort_flag, p.err) &&
            wait_all(bar_seg + 8 * (seg & 1), (seg >> 1) & 1, abort_flag, p.err);
@@ -578,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
 
       if (g.slot >= 0) {
         // a part: whoever arrives last joins, within its group of parts and then among the groups:
-        //   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M),  M = max_k lse_k
+        //   o = sum_k l_k 2^(m_k - M) o_k / sum_k l_k 2^(m_k - M),  M = max_k m_k
         const int first = cta - g.part, groups = (g.parts + kJoinFew - 1) / kJoinFew;
         int base = group_base(g, kJoinFew), stride = 1, n = min(kJoinFew, g.parts - base);
 #pragma unroll 1
@@ -595,15 +594,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
 #pragma unroll 1
           for (int i = t_key; i < g.rows * kVecs; i += 128) {
             const int r = i / kVecs, c = i % kVecs;
-            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, sum = 0.0f;
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            m = -INFINITY;
+            sum = 0.0f;
 #pragma unroll 1
             for (int k0 = 0; k0 < n; k0 += kBatch) {
-              float l2[kBatch], v[kBatch][4];
+              float2 l2[kBatch];
+              float v[kBatch][4];
 #pragma unroll
               for (int k = 0; k < kBatch; ++k) {
                 const bool in = k0 + k < n;
                 const int sl = slot_of(first, base + min(k0 + k, n - 1) * stride);
-                l2[k] = in ? __ldcg(p.part_lse + sl * kRows + r) : -INFINITY;
+                l2[k] = in ? __ldcg(p.part_sum + sl * kRows + r) : make_float2(-INFINITY, 0.0f);
                 get4(v[k], in ? __ldcg(reinterpret_cast<const float4*>(p.part + (static_cast<long long>(sl) * kRows + r) * HD) + c)
                               : make_float4(0.f, 0.f, 0.f, 0.f));
               }
@@ -611,19 +613,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
             }
             const float inv = join_inv(sum);
             const float4 o = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
-            lse2 = join_lse(m, sum);
             if (to >= 0) {
               reinterpret_cast<float4*>(p.part + (static_cast<long long>(to) * kRows + r) * HD)[c] = o;
-              if (c == 0) s_inv[r] = lse2;
+              if (c == 0) reinterpret_cast<float2*>(s_sum)[r] = make_float2(m, sum);
             } else {
               const long long orow = static_cast<long long>(g.begin + g.i0 + r / p.group) * p.heads + g.head * p.group + r % p.group;
               reinterpret_cast<uint2*>(static_cast<T*>(p.out) + orow * HD)[c] = make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
-              if (c == 0 && p.lse != nullptr) p.lse[orow] = lse2 * 0.69314718055994531f;
+              if (c == 0 && p.lse != nullptr) p.lse[orow] = join_lse(m, sum) * 0.69314718055994531f;
             }
           }
-          if (to >= 0) {  // the group's log-sum-exps have been read: its first slot takes the joined ones
+          if (to >= 0) {  // the group's sums have been read: its first slot takes the joined ones
             softmax_sync();
-            if (t_key < g.rows) p.part_lse[to * kRows + t_key] = s_inv[t_key];
+            if (t_key < g.rows) p.part_sum[to * kRows + t_key] = reinterpret_cast<const float2*>(s_sum)[t_key];
           }
           if (to < 0) break;
           base = 0;
@@ -657,8 +658,8 @@ cudaError_t launch(TreeParams& p, cudaStream_t stream) {
 cudaError_t launch_tree_few(TreeParams& p, const fl_tree_attention_args& a, cudaStream_t stream) {
   p.grid = kCtasPerSm * sm_count();
   p.tile_tokens = kRows / p.group;
-  p.part_lse = p.part + 2LL * p.grid * kRows * a.head_dim;
-  p.arrived = reinterpret_cast<unsigned long long*>(p.part_lse + 2LL * p.grid * kRows);
+  p.part_sum = reinterpret_cast<float2*>(p.part + 2LL * p.grid * kRows * a.head_dim);
+  p.arrived = reinterpret_cast<unsigned long long*>(p.part_sum + 2LL * p.grid * kRows);
   if (!encode_tree_maps(p, a, kBN)) return cudaErrorInvalidValue;
   if (a.dtype == FL_DTYPE_F16) return a.head_dim == 64 ? launch<__half, 64>(p, stream) : launch<__half, 128>(p, stream);
   return a.head_dim == 64 ? launch<__nv_bfloat16, 64>(p, stream) : launch<__nv_bfloat16, 128>(p, stream);
