@@ -25,6 +25,7 @@
 // the measured copy rate; one request of 777 keys, 8 heads of 64: 9.9 us.
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <string>
 
@@ -379,7 +380,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
     // this thread's key in a P buffer: kRows elements, 16-byte chunks swizzled as the product reads them
     const uint32_t p_row = s_p + t_key * (kRows * 2);
     const int swz = (t_key >> 2) & 1;
-    constexpr float kNone = -3.0e38f;  // reference of a row that has seen nothing
+    // Reference of a row that has seen nothing: no finite score is below it
+    // (-infinity would turn hidden scores into NaN).
+    constexpr float kNone = -FLT_MAX;
     int js = 0, seg = 0;               // tiles and segments so far
     // A wait that gives up clears ok. The four warps meet at barriers, so none
     // may leave alone: they look at each other's ok where they meet.

@@ -82,10 +82,11 @@ def test_scales(cuda, sm_scale, words, dim, tokens, heads, kv_heads):
 
 @pytest.mark.parametrize("tokens,heads,kv_heads", ROWS)
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("dtype,low,score", [(torch.float16, 60000.0, 1.0), (torch.bfloat16, 2.0 ** 64, 2.0 ** -30)])
+@pytest.mark.parametrize("dtype,low,score", [(torch.float16, 60000.0, 1.0), (torch.bfloat16, 2.0 ** 64, 2.0 ** -30),
+                                             (torch.bfloat16, 2.0 ** 64, 1.296875 / 2)])
 @pytest.mark.parametrize("n", [300, 5000])
 def test_equal_lowest_scores_average(cuda, n, dtype, low, score, dim, tokens, heads, kv_heads):
-    """Equal scores as low as a type holds them are scores, not masks: a row gives the mean of the values it sees,
+    """Equal scores as low as a type (and, last, fp32 in base 2) holds them are scores, not masks: a row gives the mean of the values it sees,
     whether or not the unit is cut into parts. Equal probabilities: only sums in fp32 and the result's rounding are off."""
     c = Case(cuda, [(n, tokens)], heads, kv_heads, dim, 16, dtype)
     c.q[:] = 0
