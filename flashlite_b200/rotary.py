@@ -62,21 +62,27 @@ def rotary_table(positions: int, rot_dim: int, base: float = 10000.0, scaling: s
 
 
 class _Rotary(torch.autograd.Function):
+    """Rotation, or with ``inverse`` its gradient. The rotation is linear, so that each is the other's gradient, and
+    gradients of any order are the same two calls."""
+
     @staticmethod
-    def forward(ctx, q, k, table, positions, interleaved, layout):
+    def forward(ctx, q, k, table, positions, interleaved, layout, inverse):
         ctx.save_for_backward(table, positions)
-        ctx.interleaved, ctx.layout = interleaved, layout
-        return rotary(q, k, table, positions, interleaved, layout)
+        ctx.interleaved, ctx.layout, ctx.inverse = interleaved, layout, inverse
+        return (rotary_backward if inverse else rotary)(q, k, table, positions, interleaved, layout)
 
     @staticmethod
     def backward(ctx, dq, dk):
         table, positions = ctx.saved_tensors
-        dq, dk = (d if d.stride(-1) == 1 else d.contiguous() for d in (dq, dk))
-        dq, dk = rotary_backward(dq, dk, table, positions, ctx.interleaved, ctx.layout)
-        return dq, dk, None, None, None, None
+        dq, dk = (d if d is None or d.stride(-1) == 1 else d.contiguous() for d in (dq, dk))
+        dq, dk = _Rotary.apply(dq, dk, table, positions, ctx.interleaved, ctx.layout, not ctx.inverse)
+        return dq, dk, None, None, None, None, None
 
 
-def rotary_embedding(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, positions: torch.Tensor | None = None,
-                     interleaved: bool = False, layout: str = "bhnd") -> tuple[torch.Tensor, torch.Tensor]:
-    """Differentiable ``rotary(q, k, table, positions)``; ``layout`` defaults to that of ``flash_attention``."""
-    return _Rotary.apply(q, k, table, positions, interleaved, layout)
+def rotary_embedding(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positions: torch.Tensor | None = None,
+                     interleaved: bool = False, layout: str = "bhnd") -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Differentiable (any order) ``rotary(q, k, table, positions)``; ``layout`` defaults to that of
+    ``flash_attention``. The table gets no gradient: one that asks for it is refused."""
+    if table.requires_grad and torch.is_grad_enabled():
+        raise ValueError("rotary_embedding has no gradient of the table: pass table.detach()")
+    return _Rotary.apply(q, k, table, positions, interleaved, layout, False)
