@@ -5,8 +5,9 @@ returns softmax(sm_scale * q k^T [causal mask]) v for ``[B, H, N, 64]`` (or,
 with ``layout="bnhd"``, ``[B, N, H, 64]``) fp16 CUDA tensors and is
 differentiable: the forward is ``forward_flash2_ex`` with the
 row log-sum-exp kept for backward, the backward is ``backward_flash2``
-(tcgen05 FA2 backward). Neither has a reference counterpart: the reference
-module is forward-only.
+(tcgen05 FA2 backward). A gradient of a gradient is not there and raises an
+error. Neither has a reference counterpart: the reference module is
+forward-only.
 """
 from __future__ import annotations
 
@@ -26,6 +27,7 @@ class _FlashAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
         dq, dk, dv = backward_flash2(q, k, v, out, dout.contiguous(), lse, ctx.sm_scale, ctx.is_causal,
