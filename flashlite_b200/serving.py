@@ -9,9 +9,11 @@ lengths, all on the device. One step is::
         out = cache.attend(layer, q, k, v, table, step)     # q, k, v of the new tokens
     cache.commit(step, kept)                                # how many each request keeps
 
-None of these waits for the GPU. With drafted trees, ``commit`` also takes the
-kept path of each request, whose keys and values move next to the cached ones.
-No reference counterpart: the reference has no cache.
+None of these waits for the GPU, and the state is updated where it lies, so that
+a step captured into a CUDA graph goes on from replay to replay (``release``
+waits, and is called between replays). With drafted trees, ``commit`` also takes
+the kept path of each request, whose keys and values move next to the cached
+ones. No reference counterpart: the reference has no cache.
 """
 from __future__ import annotations
 
@@ -48,21 +50,24 @@ class PagedCache:
         self.layers, self.page_size, self.layout = layers, page_size, layout
         # one block more than is given out: copies that are none land there (commit)
         self.spare = num_blocks * page_size
-        self.k = [torch.zeros((num_blocks + 1, *shape, head_dim), dtype=dtype, device=device) for _ in range(layers)]
-        self.v = [torch.zeros_like(k) for k in self.k]
-        ints = dict(dtype=torch.int32, device=device)
-        self.block_table = torch.zeros((requests, max_blocks), **ints)
-        self.context_lens = torch.zeros(requests, **ints)
-        self.held_blocks = torch.zeros(requests, **ints)
-        self.free_blocks = torch.arange(num_blocks - 1, -1, -1, **ints)
-        self.num_free = torch.full((1,), num_blocks, **ints)
+        with torch.inference_mode(False):  # a cache made in that mode can be written outside of it
+            self.k = [torch.zeros((num_blocks + 1, *shape, head_dim), dtype=dtype, device=device) for _ in range(layers)]
+            self.v = [torch.zeros_like(k) for k in self.k]
+            ints = dict(dtype=torch.int32, device=device)
+            self.block_table = torch.zeros((requests, max_blocks), **ints)
+            self.context_lens = torch.zeros(requests, **ints)
+            self.held_blocks = torch.zeros(requests, **ints)
+            self.free_blocks = torch.arange(num_blocks - 1, -1, -1, **ints)
+            self.num_free = torch.full((1,), num_blocks, **ints)
 
     def plan(self, cu_seqlens: torch.Tensor, total_tokens: int, parents: torch.Tensor | None = None,
              mask_words: int = 0) -> Step:
         """Blocks, slots and positions for the new tokens ``cu_seqlens[b]:cu_seqlens[b+1]`` of each request."""
-        slots, positions, admitted, self.num_free, self.held_blocks, mask = plan_cache_step(
+        slots, positions, admitted, num_free, held_blocks, mask = plan_cache_step(
             self.context_lens, cu_seqlens, self.block_table, self.held_blocks, self.free_blocks, self.num_free,
             total_tokens, self.page_size, parents=parents, mask_words=mask_words)
+        self.num_free.copy_(num_free)
+        self.held_blocks.copy_(held_blocks)
         return Step(cu_seqlens, slots, positions, admitted, mask)
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, step: Step,
@@ -95,12 +100,12 @@ class PagedCache:
                     cache[tb, tr] = cache[sb, sr]
                 else:
                     cache[tb, :, tr] = cache[sb, :, sr]
-        self.context_lens = self.context_lens + kept
+        self.context_lens += kept
 
     def release(self, request: int) -> None:
         """Gives a finished request's blocks back. Reads its length, so it waits for the GPU."""
         held, free = int(self.held_blocks[request]), int(self.num_free)
         self.free_blocks[free:free + held] = self.block_table[request, :held]
-        self.num_free = self.num_free + held
+        self.num_free += held
         self.context_lens[request] = 0
         self.held_blocks[request] = 0
