@@ -153,9 +153,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_kernel(const __
                         : a.positions_64 ? static_cast<const int64_t*>(a.positions)[pi]
                                          : static_cast<const int32_t*>(a.positions)[pi];
   const bool known = pos >= 0 && pos < a.table_rows;
-  if (!known && a.rot > 0 && u0 == 0 && p.err) atomicOr(p.err, kDevErrIndex);
   long long kc = 0, vc = 0;  // the token's row in the caches
   bool cached = false;
+  bool sound = known || a.rot == 0;
   if (a.slots != nullptr) {
     const long long slot = a.slots[t];
     cached = slot >= 0 && slot < a.cache_blocks * a.page_size;
@@ -166,10 +166,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_kernel(const __
       const long long r = slot - blk * a.page_size;
       kc = blk * a.k_out_stride[0] + r * a.k_out_stride[1];
       vc = blk * a.v_out_stride[0] + r * a.v_out_stride[1];
-    } else if (slot != -1 && u0 == 0 && p.err) {
-      atomicOr(p.err, kDevErrIndex);
+    } else {
+      // a token that the cache step refused: its position may be anywhere
+      sound = slot == -1;
     }
   }
+  if (!sound && u0 == 0 && p.err) atomicOr(p.err, kDevErrIndex);
 
   T* k_out = static_cast<T*>(a.k_out) + (a.slots == nullptr ? row_of(a.k_out_stride, b, n, 0) : kc);
   T* v_out = static_cast<T*>(a.v_out) + vc;

@@ -179,7 +179,8 @@ enum fl_dtype {
  * NaN in the rotated columns. Outputs may be the inputs themselves.
  * With slots != NULL ([batch * length] int64) the rotated k and the unchanged
  * v go to row `slot` of k_out and v_out, caches of cache_blocks blocks of
- * page_size rows with strides {block, row, head}; slot -1 writes nothing.
+ * page_size rows with strides {block, row, head}; slot -1 writes nothing, and
+ * a position outside the table is not recorded there (a refused token's).
  * Distinct tokens need distinct slots.
  */
 typedef struct fl_rotary_args {
