@@ -76,7 +76,9 @@ struct Request {
 __device__ __forceinline__ Request request_of(const TreeParams& p, int begin, int end, int ctx, bool report) {
   Request r;
   const long long room = static_cast<long long>(p.table_cols) << p.page_shift;
-  r.room = room > 0x3fffffff ? 0x3fffffff : static_cast<int>(room);
+  const bool part = ctx != -1;  // a request that takes no part (a refused one) sees no key
+  if (!part) ctx = 0;
+  r.room = !part ? 0 : room > 0x3fffffff ? 0x3fffffff : static_cast<int>(room);
   bool sound = true;
   r.begin = begin;
   r.count = end - begin;
@@ -89,7 +91,7 @@ __device__ __forceinline__ Request request_of(const TreeParams& p, int begin, in
     sound = false;
     r.ctx = ctx < 0 ? 0 : r.room;
   }
-  if (r.count > r.room - r.ctx) sound = false;  // the new tokens past the table's end are not visible
+  if (part && r.count > r.room - r.ctx) sound = false;  // the new tokens past the table's end are not visible
   if (!sound && report) atomicOr(p.err, kDevErrIndex);
   return r;
 }
@@ -278,7 +280,7 @@ struct Scheduler {
     r.begin = __shfl_sync(0xffffffffu, mine.begin, b);
     r.count = __shfl_sync(0xffffffffu, mine.count, b);
     r.ctx = __shfl_sync(0xffffffffu, mine.ctx, b);
-    r.room = mine.room;
+    r.room = __shfl_sync(0xffffffffu, mine.room, b);
     const uint32_t ph = __shfl_sync(0xffffffffu, per_head, b);
     h = static_cast<int>(static_cast<uint32_t>(rest) / ph);
     rest -= h * ph;

@@ -32,6 +32,7 @@ class Step(NamedTuple):
     positions: torch.Tensor
     admitted: torch.Tensor
     tree_mask: torch.Tensor | None
+    context_lens: torch.Tensor | None = None  # cached tokens, -1 for a refused request: as attention takes them
 
 
 class PagedCache:
@@ -68,15 +69,17 @@ class PagedCache:
             total_tokens, self.page_size, parents=parents, mask_words=mask_words)
         self.num_free.copy_(num_free)
         self.held_blocks.copy_(held_blocks)
-        return Step(cu_seqlens, slots, positions, admitted, mask)
+        return Step(cu_seqlens, slots, positions, admitted, mask, torch.where(admitted, self.context_lens, -1))
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, step: Step,
                interleaved: bool = False, sm_scale: float = 0.0) -> torch.Tensor:
-        """Rotates ``q`` and ``k``, appends ``k`` and ``v`` to the layer's cache and attends to it."""
+        """Rotates ``q`` and ``k``, appends ``k`` and ``v`` to the layer's cache and attends to it. The rows of a refused
+        request are 0."""
+        lens = self.context_lens if step.context_lens is None else step.context_lens
         q = rotary_append(q, k, v, table, step.positions, step.slots, self.k[layer], self.v[layer],
                           interleaved=interleaved, layout=self.layout)
-        out, _ = tree_attention(q, self.k[layer], self.v[layer], self.block_table, self.context_lens,
-                                step.cu_seqlens, tree_mask=step.tree_mask, sm_scale=sm_scale, layout=self.layout)
+        out, _ = tree_attention(q, self.k[layer], self.v[layer], self.block_table, lens, step.cu_seqlens,
+                                tree_mask=step.tree_mask, sm_scale=sm_scale, layout=self.layout)
         return out
 
     def commit(self, step: Step, kept: torch.Tensor, path: torch.Tensor | None = None) -> None:
