@@ -43,7 +43,7 @@ struct Request {
 };
 
 // A request's share of the arithmetic above. Lengths out of range count as
-// none and are recorded.
+// none and are recorded; the request is refused and keeps the blocks it holds.
 __device__ __forceinline__ Request request_from(const PlanParams& p, int ctx, int begin, int end, int held, bool report) {
   const fl_plan_args& a = p.a;
   Request r;
@@ -53,7 +53,8 @@ __device__ __forceinline__ Request request_from(const PlanParams& p, int ctx, in
                      r.ctx <= 0x7fffffff - (end - r.begin) - static_cast<int>(a.page_size);
   if (!sound) {
     if (report && p.err) atomicOr(p.err, kDevErrIndex);
-    r.ctx = r.begin = r.count = r.have = r.need = 0;
+    r.ctx = r.begin = r.count = r.need = 0;
+    r.have = held;
     r.fits = false;
     return r;
   }

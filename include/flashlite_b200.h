@@ -210,10 +210,14 @@ int fl_rotary(const fl_rotary_args* args, void* stream);
  * free_blocks[0 .. num_free[0] - 1], requests in order, and entered in its
  * row of block_table (requests x table_cols, row stride table_stride), in
  * place. A request whose blocks do not fit (its row, or what is free after
- * the requests before it) is refused: admitted[b] = 0, its row unchanged,
- * its slots -1. Out: slots and positions of the `tokens` new tokens (tokens
- * past cu_seqlens[requests] get slot -1, position 0), admitted and
- * held_after [requests], num_free_after [1].
+ * the requests before it) is refused: admitted[b] = 0, its row and the blocks
+ * it holds unchanged, its slots -1; so is one whose length or offsets are out
+ * of range. What a request needs counts against those after it even if it is
+ * refused for lack of free blocks: once one does not fit, later ones get no
+ * new blocks in this step (a long prompt does not starve while short requests
+ * pass it). Out: slots and positions of the `tokens` new tokens (tokens past
+ * cu_seqlens[requests] get slot -1, position 0), admitted and held_after
+ * [requests], num_free_after [1].
  * Trees: parents[t] is the index, within its request, of the token that t
  * follows, smaller than its own, or -1 for the last cached token; the
  * position of t is then context + depth, and tree_mask (tokens x mask_words
