@@ -259,6 +259,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
           if (lane == 0) mbar_arrive(bar_count + 8 * (g.slot & 1));
         }
       }
+      clear_padding<T, HD>(p, cta, p.grid, lane);
     } else if (warp == 0 || warp == 2) {
       // ======================= K (and Q) producer, V producer =======================
       const bool is_k = warp == 0;
@@ -700,8 +701,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attention_kernel(co
         }
       }
     }
-
-    clear_padding<T, HD>(p, cta * 4 + (warp - 4), p.grid * 4, lane);
   }
 
   __syncthreads();

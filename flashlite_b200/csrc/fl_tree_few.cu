@@ -272,6 +272,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
       if (worker == 0)
         for (int i = max(seg - 2, 0); i < seg; ++i) mbar_wait_quiet(bar_qfull + 8 * (i & 1), (i >> 1) & 1);
     }
+    __syncwarp();
+    if (worker > 0) clear_padding<T, HD>(p, cta, p.grid, lane);
   } else if (warp == 1) {
     // ======================= S^T = K Q^T =======================
     constexpr uint32_t idesc = make_idesc_f16_f32(kBN, kRows, false, false, kBf16);  // K-major A (K) and B (Q)
@@ -636,8 +638,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __
         }
       }
     }
-
-    clear_padding<T, HD>(p, cta * 4 + (warp - 4), p.grid * 4, lane);
   }
 
   __syncthreads();

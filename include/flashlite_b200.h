@@ -258,8 +258,9 @@ int fl_plan_cache_step(const fl_plan_args* args, void* stream);
  * outside the visible keys, NaN included, does not enter a row. out (tokens x
  * heads x head_dim, contiguous); lse [tokens, heads] fp32 or NULL: natural-log
  * log-sum-exp of the scaled scores. A row without a visible key gives 0 and
- * -inf, and so do all rows of a request with context_lens[b] == -1, which
- * takes no part (one that fl_plan_cache_step refused: its row of the table
+ * -inf, and so do rows of q that belong to no request (or to one whose
+ * offsets are out of range) and those of a request with context_lens[b] == -1,
+ * which takes no part (one that fl_plan_cache_step refused: its row of the table
  * names no blocks for its new tokens). sm_scale == 0 means 1/sqrt(head_dim). workspace: device memory of at
  * least fl_tree_attention_workspace_size() bytes, 16-byte aligned, for this
  * call alone until it has run. At most 4096 requests.
