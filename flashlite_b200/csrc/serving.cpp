@@ -62,6 +62,13 @@ Tensor fresh(torch::IntArrayRef sizes, torch::ScalarType type) {
   return Outputs(bytes).take(sizes, type);
 }
 
+// A tensor of the caller's that a call has written: torch is told, as by its own
+// in-place operations, so that autograd finds a saved tensor changed. (Those of
+// inference mode keep no version.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 bool given(const OptTensor& t) { return t.has_value() && t.value().defined(); }
 
 int dtype_of(const Tensor& t, bool with_fp32, const char* who) {
@@ -196,6 +203,8 @@ std::tuple<Tensor, OptTensor> rotary_any(const Tensor& q, const OptTensor& k, co
   a.interleaved = interleaved;
   a.inverse = inverse;
   check_status(fl_rotary(&a, stream_of(q)));
+  if (given(out_q)) written(oq);
+  if (given(out_k)) written(*ok);
   return {oq, ok};
 }
 
@@ -269,6 +278,9 @@ Tensor rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   a.interleaved = interleaved;
   if (a.length == 0) return oq;
   check_status(fl_rotary(&a, stream_of(q)));
+  written(k_cache);
+  written(v_cache);
+  if (given(out_q)) written(oq);
   return oq;
 }
 
@@ -332,6 +344,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor> plan_cache_step(
   a.page_size = page_size;
   a.mask_words = mask_words;
   check_status(fl_plan_cache_step(&a, stream_of(context_lens)));
+  written(block_table);
   return {slots, positions, admitted, left, held, mask};
 }
 
@@ -405,6 +418,7 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor& q, const Tensor& k_ca
   put(a.v_stride, cv.stride);
   a.sm_scale = static_cast<float>(sm_scale);
   check_status(fl_tree_attention(&a, stream_of(q)));
+  if (given(out)) written(out_tensor);
   return {out_tensor, lse};
 }
 
