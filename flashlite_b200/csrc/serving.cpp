@@ -20,7 +20,16 @@ namespace {
 using torch::Tensor;
 using OptTensor = std::optional<Tensor>;
 
-void check_status(int status) {
+// Makes a call of the C ABI and turns its status into an error. The launch
+// blocks while the device's launch queue is full; other Python threads keep
+// running meanwhile (the error text is thread-local).
+template <typename Args>
+void launch(int (*fn)(const Args*, void*), const Args& args, void* stream) {
+  int status;
+  {
+    pybind11::gil_scoped_release no_gil;
+    status = fn(&args, stream);
+  }
   TORCH_CHECK(status == FL_OK, "flashlite_b200: ", fl_status_str(status), ": ", fl_last_error());
 }
 
@@ -202,7 +211,7 @@ std::tuple<Tensor, OptTensor> rotary_any(const Tensor& q, const OptTensor& k, co
   set_positions(a, positions, q);
   a.interleaved = interleaved;
   a.inverse = inverse;
-  check_status(fl_rotary(&a, stream_of(q)));
+  launch(fl_rotary, a, stream_of(q));
   if (given(out_q)) written(oq);
   if (given(out_k)) written(*ok);
   return {oq, ok};
@@ -277,7 +286,7 @@ Tensor rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   set_positions(a, positions, q);
   a.interleaved = interleaved;
   if (a.length == 0) return oq;
-  check_status(fl_rotary(&a, stream_of(q)));
+  launch(fl_rotary, a, stream_of(q));
   written(k_cache);
   written(v_cache);
   if (given(out_q)) written(oq);
@@ -343,7 +352,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor> plan_cache_step(
   a.free_capacity = free_blocks.size(0);
   a.page_size = page_size;
   a.mask_words = mask_words;
-  check_status(fl_plan_cache_step(&a, stream_of(context_lens)));
+  launch(fl_plan_cache_step, a, stream_of(context_lens));
   written(block_table);
   return {slots, positions, admitted, left, held, mask};
 }
@@ -417,7 +426,7 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor& q, const Tensor& k_ca
   put(a.k_stride, ck.stride);
   put(a.v_stride, cv.stride);
   a.sm_scale = static_cast<float>(sm_scale);
-  check_status(fl_tree_attention(&a, stream_of(q)));
+  launch(fl_tree_attention, a, stream_of(q));
   if (given(out)) written(out_tensor);
   return {out_tensor, lse};
 }
