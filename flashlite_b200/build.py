@@ -94,6 +94,23 @@ def build_library(verbose: bool = False) -> Path:
     return LIB
 
 
+def loaded_cxx_runtime(maps=Path("/proc/self/maps")) -> list[str]:
+    """Path of the C++ runtime that torch has loaded into this process, to link against.
+
+    A compiler that finds only libstdc++.a would link a second runtime in, whose streams do not work with the first
+    one's locales (a number in an error text crashes). Empty where the process does not tell: the compiler's default.
+    """
+    try:
+        lines = Path(maps).read_text().splitlines()
+    except OSError:
+        return []
+    for line in lines:
+        path = line.split(maxsplit=5)[-1]
+        if os.path.basename(path).startswith("libstdc++.so.6"):
+            return [path]
+    return []
+
+
 def build_binding(verbose: bool = False) -> Path:
     """Compile the torch binding (BINDING_SOURCES) against libflashlite_b200.so."""
     import torch
@@ -123,10 +140,7 @@ def build_binding(verbose: bool = False) -> Path:
            *[f"-L{p}" for p in libdirs], f"-L{PKG}",
            "-lflashlite_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
            "-ltorch_python", "-lcudart",
-           # torch's own C++ runtime, by file name: a compiler that finds only
-           # libstdc++.a would link a second one in, whose streams do not work
-           # with the first one's locales (a number in an error text crashes)
-           "-l:libstdc++.so.6",
+           *loaded_cxx_runtime(),
            "-Wl,-rpath,$ORIGIN"]
     out = _run(cmd, BUILD / "binding.log")
     if verbose:
