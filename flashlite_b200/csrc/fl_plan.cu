@@ -250,8 +250,54 @@ int plan(const fl_plan_args* args, void* stream) {
   return e == cudaSuccess ? FL_OK : cuda_fail(e, "plan launch");
 }
 
+// A step's results into the state they follow, a thread for each request. A
+// kernel of its own: every block of the first one reads all of the state.
+struct SettleParams {
+  const int32_t* context_lens;
+  const uint8_t* admitted;
+  const int32_t* held_after;
+  const int32_t* num_free_after;
+  int32_t* held_blocks;
+  int32_t* num_free;
+  int32_t* attention_lens;
+  int requests;
+};
+
+__global__ void __launch_bounds__(kThreads) settle_kernel(const __grid_constant__ SettleParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int b = blockIdx.x * kThreads + threadIdx.x;
+  if (b == 0) p.num_free[0] = p.num_free_after[0];
+  if (b >= p.requests) return;
+  p.held_blocks[b] = p.held_after[b];
+  p.attention_lens[b] = p.admitted[b] ? p.context_lens[b] : -1;
+}
+
+int settle(const SettleParams& p, int64_t requests, void* stream) {
+  if (requests < 0) return fail(FL_ERR_INVALID_ARGUMENT, "negative size");
+  if (requests > kMaxRequests) return fail(FL_ERR_UNSUPPORTED, "at most 16384 requests");
+  if (!p.num_free_after || !p.num_free ||
+      (requests > 0 && (!p.context_lens || !p.admitted || !p.held_after || !p.held_blocks || !p.attention_lens)))
+    return fail(FL_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  const int st = check_device();
+  if (st != FL_OK) return st;
+  const int blocks = std::max(1, (p.requests + kThreads - 1) / kThreads);
+  const cudaError_t e = launch_pdl(settle_kernel, blocks, kThreads, 0, static_cast<cudaStream_t>(stream), p);
+  return e == cudaSuccess ? FL_OK : cuda_fail(e, "settle launch");
+}
+
 }  // namespace
 }  // namespace fl
+
+extern "C" int fl_settle_step(const int32_t* context_lens, const uint8_t* admitted, const int32_t* held_after,
+                              const int32_t* num_free_after, int32_t* held_blocks, int32_t* num_free,
+                              int32_t* attention_lens, int64_t requests, void* stream) {
+  return fl::guarded([&] {
+    return fl::settle({context_lens, admitted, held_after, num_free_after, held_blocks, num_free, attention_lens,
+                       static_cast<int>(requests)},
+                      requests, stream);
+  });
+}
 
 extern "C" int fl_plan_cache_step(const fl_plan_args* args, void* stream) {
   return fl::guarded([&] { return fl::plan(args, stream); });

@@ -23,12 +23,12 @@ using OptTensor = std::optional<Tensor>;
 // Makes a call of the C ABI and turns its status into an error. The launch
 // blocks while the device's launch queue is full; other Python threads keep
 // running meanwhile (the error text is thread-local).
-template <typename Args>
-void launch(int (*fn)(const Args*, void*), const Args& args, void* stream) {
+template <typename Call>
+void launch(Call&& call) {
   int status;
   {
     pybind11::gil_scoped_release no_gil;
-    status = fn(&args, stream);
+    status = call();
   }
   TORCH_CHECK(status == FL_OK, "flashlite_b200: ", fl_status_str(status), ": ", fl_last_error());
 }
@@ -211,7 +211,7 @@ std::tuple<Tensor, OptTensor> rotary_any(const Tensor& q, const OptTensor& k, co
   set_positions(a, positions, q);
   a.interleaved = interleaved;
   a.inverse = inverse;
-  launch(fl_rotary, a, stream_of(q));
+  launch([&, stream = stream_of(q)] { return fl_rotary(&a, stream); });
   if (given(out_q)) written(oq);
   if (given(out_k)) written(*ok);
   return {oq, ok};
@@ -286,7 +286,7 @@ Tensor rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   set_positions(a, positions, q);
   a.interleaved = interleaved;
   if (a.length == 0) return oq;
-  launch(fl_rotary, a, stream_of(q));
+  launch([&, stream = stream_of(q)] { return fl_rotary(&a, stream); });
   written(k_cache);
   written(v_cache);
   if (given(out_q)) written(oq);
@@ -352,9 +352,37 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor> plan_cache_step(
   a.free_capacity = free_blocks.size(0);
   a.page_size = page_size;
   a.mask_words = mask_words;
-  launch(fl_plan_cache_step, a, stream_of(context_lens));
+  launch([&, stream = stream_of(context_lens)] { return fl_plan_cache_step(&a, stream); });
   written(block_table);
   return {slots, positions, admitted, left, held, mask};
+}
+
+// A step's held blocks and free count into the state that they follow; returns
+// the lengths that attention takes.
+Tensor settle_step(const Tensor& context_lens, const Tensor& held_blocks, const Tensor& num_free, const Tensor& admitted,
+                   const Tensor& held_after, const Tensor& free_after) {
+  TORCH_CHECK(context_lens.is_cuda(), "All tensors must be on CUDA");
+  const torch::Device dev = context_lens.device();
+  const int64_t n = context_lens.size(0);
+  check_ints(context_lens, dev, torch::kInt, 1, "context_lens");
+  check_ints(held_blocks, dev, torch::kInt, 1, "held_blocks");
+  check_ints(num_free, dev, torch::kInt, 1, "num_free");
+  check_ints(admitted, dev, torch::kBool, 1, "admitted");
+  check_ints(held_after, dev, torch::kInt, 1, "held_after");
+  check_ints(free_after, dev, torch::kInt, 1, "free_after");
+  TORCH_CHECK(held_blocks.size(0) == n && admitted.size(0) == n && held_after.size(0) == n,
+              "held_blocks, admitted and held_after must hold one value for each request");
+  TORCH_CHECK(num_free.size(0) == 1 && free_after.size(0) == 1, "num_free and free_after must hold one value");
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor lens = fresh({n}, torch::kInt);
+  launch([&, stream = stream_of(context_lens)] {
+    return fl_settle_step(context_lens.data_ptr<int32_t>(), reinterpret_cast<const uint8_t*>(admitted.data_ptr<bool>()),
+                          held_after.data_ptr<int32_t>(), free_after.data_ptr<int32_t>(), held_blocks.data_ptr<int32_t>(),
+                          num_free.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), n, stream);
+  });
+  written(held_blocks);
+  written(num_free);
+  return lens;
 }
 
 // Attention of new tokens over the paged cache. Returns (out, lse).
@@ -426,7 +454,7 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor& q, const Tensor& k_ca
   put(a.k_stride, ck.stride);
   put(a.v_stride, cv.stride);
   a.sm_scale = static_cast<float>(sm_scale);
-  launch(fl_tree_attention, a, stream_of(q));
+  launch([&, stream = stream_of(q)] { return fl_tree_attention(&a, stream); });
   if (given(out)) written(out_tensor);
   return {out_tensor, lse};
 }
@@ -449,6 +477,10 @@ void bind_serving(pybind11::module_& m) {
         py::arg("context_lens"), py::arg("cu_seqlens"), py::arg("block_table"), py::arg("held_blocks"), py::arg("free_blocks"),
         py::arg("num_free"), py::arg("total_tokens"), py::arg("page_size"), py::arg("parents") = py::none(),
         py::arg("mask_words") = 0);
+  m.def("settle_step", &settle_step,
+        "Held blocks and free count of a step into the cache's state; returns the lengths that attention takes",
+        py::arg("context_lens"), py::arg("held_blocks"), py::arg("num_free"), py::arg("admitted"), py::arg("held_after"),
+        py::arg("free_after"));
   m.def("tree_attention", &tree_attention, "Attention of new tokens over a paged cache; returns (out, lse)",
         py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"), py::arg("context_lens"),
         py::arg("cu_seqlens"), py::arg("tree_mask") = py::none(), py::arg("sm_scale") = 0.0,

@@ -41,6 +41,9 @@ rotary also fp32):
   num_free, total_tokens, page_size, parents=None, mask_words=0) -> (slots, positions,
   admitted, num_free, held_blocks, tree_mask)`` gives new tokens their blocks, slots, positions
   and, for trees of drafted tokens, ancestor masks, on the device.
+* ``settle_step(context_lens, held_blocks, num_free, admitted, held_after, free_after) -> attention_lens`` puts
+  its results into the tensors that it read, for a cache whose state stays where it is, and gives the lengths
+  that ``tree_attention`` takes: -1 for a refused request.
 * ``rotary_append(q, k, v, table, positions, slots, k_cache, v_cache,
   interleaved=False, layout="bnhd", out_q=None) -> q`` rotates q and k and writes k
   and v to their slots.
@@ -49,7 +52,7 @@ rotary also fp32):
   lse)`` attends the new tokens to the paged cache; ``lse`` is ``[tokens, heads]``,
   or None unless ``return_lse``.
 
-``flashlite_b200.serving.PagedCache`` holds the state these four calls share.
+``flashlite_b200.serving.PagedCache`` holds the state these calls share.
 """
 from __future__ import annotations
 
@@ -58,7 +61,7 @@ import torch  # noqa: F401  (loads libtorch/libc10 for the binding)
 try:
     from ._C import (backward_flash2, device_error, forward_block, forward_flash2,
                      forward_flash2_ex, forward_naive, plan_cache_step, ring_finalize, rotary,
-                     rotary_append, rotary_backward, tree_attention)
+                     rotary_append, rotary_backward, settle_step, tree_attention)
 except ImportError as exc:  # pragma: no cover - exercised only on unbuilt trees
     raise ImportError(
         "flashlite_b200 native extension is not built; run `python -m flashlite_b200.build` "
@@ -67,4 +70,4 @@ except ImportError as exc:  # pragma: no cover - exercised only on unbuilt trees
 
 __all__ = ["forward_flash2", "forward_naive", "forward_flash2_ex", "forward_block", "ring_finalize",
            "backward_flash2", "device_error", "rotary", "rotary_backward", "rotary_append",
-           "plan_cache_step", "tree_attention"]
+           "plan_cache_step", "settle_step", "tree_attention"]

@@ -21,7 +21,7 @@ from typing import NamedTuple
 
 import torch
 
-from .flash_attn_wmma import plan_cache_step, rotary_append, tree_attention
+from .flash_attn_wmma import plan_cache_step, rotary_append, settle_step, tree_attention
 
 
 class Step(NamedTuple):
@@ -67,9 +67,8 @@ class PagedCache:
         slots, positions, admitted, num_free, held_blocks, mask = plan_cache_step(
             self.context_lens, cu_seqlens, self.block_table, self.held_blocks, self.free_blocks, self.num_free,
             total_tokens, self.page_size, parents=parents, mask_words=mask_words)
-        self.num_free.copy_(num_free)
-        self.held_blocks.copy_(held_blocks)
-        return Step(cu_seqlens, slots, positions, admitted, mask, torch.where(admitted, self.context_lens, -1))
+        lens = settle_step(self.context_lens, self.held_blocks, self.num_free, admitted, held_blocks, num_free)
+        return Step(cu_seqlens, slots, positions, admitted, mask, lens)
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, step: Step,
                interleaved: bool = False, sm_scale: float = 0.0) -> torch.Tensor:

@@ -245,6 +245,16 @@ typedef struct fl_plan_args {
 int fl_plan_cache_step(const fl_plan_args* args, void* stream);
 
 /*
+ * For a cache that keeps its state where it is (a captured step reads it there
+ * again): held_after and num_free_after of fl_plan_cache_step into held_blocks
+ * [requests] and num_free [1], and attention_lens[b] = context_lens[b], or -1
+ * for a refused request, as fl_tree_attention takes them.
+ */
+int fl_settle_step(const int32_t* context_lens, const uint8_t* admitted, const int32_t* held_after,
+                   const int32_t* num_free_after, int32_t* held_blocks, int32_t* num_free,
+                   int32_t* attention_lens, int64_t requests, void* stream);
+
+/*
  * Attention of new tokens over a paged cache. Row t of q (tokens x heads x
  * head_dim, strides {token, head}) is token i = t - cu_seqlens[b] of request
  * b; it sees the context_lens[b] cached keys of its request and, of the

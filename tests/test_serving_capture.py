@@ -17,7 +17,13 @@ def test_state_stays_where_it_is(monkeypatch, inference):
         return (torch.zeros(total, dtype=torch.long), torch.zeros(total, dtype=torch.int32),
                 torch.ones(n, dtype=torch.bool), num_free - n, held + 1, None)
 
+    def settle(context_lens, held, num_free, admitted, held_after, free_after):
+        held.copy_(held_after)
+        num_free.copy_(free_after)
+        return torch.where(admitted, context_lens, -1)
+
     monkeypatch.setattr(flashlite_b200.serving, "plan_cache_step", plan)
+    monkeypatch.setattr(flashlite_b200.serving, "settle_step", settle, raising=False)
     with torch.inference_mode(inference):
         cache = PagedCache(2, 8, 16, 1, 64, 4, device="cpu")
     state = lambda: (cache.context_lens, cache.held_blocks, cache.num_free, cache.free_blocks, cache.block_table)  # noqa: E731
