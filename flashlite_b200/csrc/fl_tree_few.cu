@@ -1,6 +1,9 @@
 // Attention over a paged cache for few rows: up to 16 to a unit, the tokens of
 // a request times the query heads that share a key head (decoding single
-// tokens, small trees). Same mathematics as fl_tree.cu.
+// tokens, small trees). Same mathematics and roundings as fl_tree.cu, except
+// that O is divided by the sum of all probabilities as rounded (fl_tree.cu:
+// by the sum, corrected for each tile's largest only; the threads here hold
+// the rounded ones of all rows anyway).
 //
 // Bound by the keys and values read once from memory, and for small calls by
 // latency. With S = Q K^T as a 128-row product, so few rows would leave one

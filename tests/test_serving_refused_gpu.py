@@ -9,7 +9,7 @@ from flashlite_b200 import flash_attn_wmma as fa
 from flashlite_b200.rotary import rotary_table
 from flashlite_b200.serving import PagedCache
 
-from tests.test_tree_attention_gpu import Case
+from test_tree_attention_gpu import Case
 
 pytestmark = pytest.mark.gpu
 

@@ -7,7 +7,7 @@ import torch
 
 from flashlite_b200 import flash_attn_wmma as fa
 
-from tests.test_tree_attention_gpu import Case
+from test_tree_attention_gpu import Case
 
 pytestmark = pytest.mark.gpu
 
