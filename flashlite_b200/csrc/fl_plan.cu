@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ 
   const fl_plan_args& a = p.a;
   const int nb = static_cast<int>(a.requests), total = static_cast<int>(a.tokens);
   int* s_first = smem;    // [nb] blocks needed (-1: the row is too short), then taken by the requests before (-1: refused)
-  int* s_cu = smem + nb;  // [nb + 1]
+  int* s_cu = smem + nb;  // [nb] first token, rising
   __shared__ long long s_warp[kThreads / 32];
   __shared__ int s_used;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ 
   // blocks that are not there cannot be given out
   const int free_n = max(0, min(a.num_free[0], static_cast<int>(a.free_capacity)));
 
+  bool in_order = true;
   // ---- prefix sum of the blocks needed: each thread takes a run of requests ----
   constexpr int kAhead = 4;  // requests of a thread whose loads are under way together
   for (int base = tid; base < nb; base += kAhead * kThreads) {
@@ -109,14 +110,19 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ 
       if (b >= nb) break;
       const Request r = request_from(p, ctx[i], begin[i], end[i], held[i], blockIdx.x == 0);
       s_first[b] = r.fits ? r.need : -1;
-      s_cu[b] = begin[i];
+      const bool sound = begin[i] >= 0 && end[i] >= begin[i] && end[i] <= total;
+      s_cu[b] = sound ? begin[i] : 0x7fffffff;
+      in_order &= sound;
     }
   }
-  if (tid == 0) {
-    s_used = 0;
-    s_cu[nb] = a.cu_seqlens[nb];
+  if (tid == 0) s_used = 0;
+  if (__syncthreads_or(!in_order)) {
+    // Offsets out of range: those requests begin where the next sound one does,
+    // so that the tokens' search below passes them by.
+    if (tid == 0)
+      for (int b = nb - 2; b >= 0; --b) s_cu[b] = min(s_cu[b], s_cu[b + 1]);
+    __syncthreads();
   }
-  __syncthreads();
   const int per = (nb + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, nb), b1 = min(b0 + per, nb);
   long long mine = 0;
@@ -239,9 +245,9 @@ int plan(const fl_plan_args* args, void* stream) {
   PlanParams p;
   p.a = a;
   p.err = device_error_word();
-  const int smem = static_cast<int>(2 * a.requests + 1) * 4;
+  const int smem = static_cast<int>(2 * a.requests) * 4;
   static std::atomic<bool> configured[kMaxFlagDevices];
-  cudaError_t e = ensure_smem_limit(plan_kernel, (2 * kMaxRequests + 1) * 4, configured);
+  cudaError_t e = ensure_smem_limit(plan_kernel, 2 * kMaxRequests * 4, configured);
   if (e != cudaSuccess) return cuda_fail(e, "plan launch");
   const int64_t want = std::max<int64_t>((a.tokens + kThreads - 1) / kThreads,
                                          (a.requests + kThreads / 32 - 1) / (kThreads / 32));
